@@ -30,8 +30,9 @@ extern "C" {
 
 #define TPO_B200_ABI_VERSION 1
 
-/* element types (match torch's float32 / float16 / float64) */
-enum tpo_dtype { TPO_F32 = 0, TPO_F16 = 1, TPO_F64 = 2 };
+/* element types (match torch's float32 / float16 / float64 / bfloat16; bfloat16 is
+ * taken by the token operators only: layer norm and attention) */
+enum tpo_dtype { TPO_F32 = 0, TPO_F16 = 1, TPO_F64 = 2, TPO_BF16 = 3 };
 
 /* flags for the chamfer distance arithmetic.
  * TPO_ROUND_FMA (default, 0): d = fma(dz,dz, fma(dx,dx, dy*dy)) -- bit-identical to
@@ -65,7 +66,9 @@ TPO_API int tpo_abi_version(void);
  * *flags (synchronous) and clears them if `clear` is non-zero. */
 enum tpo_device_errors {
   TPO_DEVERR_BULK_TIMEOUT = 1, /* a bulk copy's mbarrier wait gave up           */
-  TPO_DEVERR_GRID_TIMEOUT = 2  /* fps: a grid-wide step barrier wait gave up     */
+  TPO_DEVERR_GRID_TIMEOUT = 2, /* fps: a grid-wide step barrier wait gave up     */
+  TPO_DEVERR_BAD_OFFSETS = 4,  /* packed attention: offsets decrease or leave the tensor */
+  TPO_DEVERR_MMA_TIMEOUT = 8   /* packed attention: a wait inside a block gave up */
 };
 TPO_API int tpo_device_error_flags(unsigned* flags, int clear);
 
@@ -240,6 +243,74 @@ TPO_API int tpo_gather_points_fwd(int dtype, const void* points, const int64_t* 
                                   int64_t C, int64_t P, int64_t M, void* out, void* stream);
 TPO_API int tpo_gather_points_bwd(int dtype, const void* grad_out, const int64_t* idx, int64_t N,
                                   int64_t C, int64_t P, int64_t M, void* grad_points, void* stream);
+
+/* ------------------------------------------------------------------------- */
+/* Token operators: the pre-norm attention block over tokens of point clouds (no
+ * counterpart in the reference). */
+
+/* Layer norm over the last dimension of x (rows, width), row stride x_stride
+ * elements, elements of a row contiguous:
+ *   y = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(var + eps)
+ * with the biased variance; moments, sums and the affine step in fp32 (fp64 for
+ * TPO_F64), y rounded once.  weight, bias (width) have type wdtype (dtype itself,
+ * or TPO_F32 with 16-bit rows); either may be NULL.  y (rows, width) contiguous;
+ * mean, rstd (rows) fp32 (fp64 for TPO_F64), both NULL where no backward follows. */
+TPO_API int tpo_layer_norm_fwd(int dtype, int wdtype, const void* x, int64_t x_stride, const void* weight,
+                               const void* bias, int64_t rows, int64_t width, double eps, void* y,
+                               void* mean, void* rstd, void* stream);
+/* Its backward: dx (rows, width) of type dtype, dweight, dbias (width) of type
+ * wdtype, each fully written, each NULL where it is not wanted.  The column sums go
+ * through `workspace` (tpo_layer_norm_bwd_workspace_size() bytes, 16-byte
+ * aligned) in a fixed order: every run gives the same bits. */
+TPO_API size_t tpo_layer_norm_bwd_workspace_size(int dtype, int64_t rows, int64_t width);
+TPO_API int tpo_layer_norm_bwd(int dtype, int wdtype, const void* x, int64_t x_stride, const void* dy,
+                               int64_t dy_stride, const void* weight, const void* mean, const void* rstd,
+                               int64_t rows, int64_t width, void* dx, void* dweight, void* dbias,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention over packed clouds.  q (tokens_q, heads, width), k and v (tokens_k,
+ * kv_heads, width) hold the tokens of all clouds one after another; cloud i has
+ * queries [offsets_q[i], offsets_q[i+1]) and keys [offsets_k[i], offsets_k[i+1])
+ * (device arrays of clouds + 1 non-decreasing int64; decreasing or outside values
+ * are clamped and raise TPO_DEVERR_BAD_OFFSETS, the results are then undefined).
+ * heads is a multiple of kv_heads; query head h reads kv head h / (heads / kv_heads).
+ * causal: with nq queries and nk keys, query i sees keys j <= i + nk - nq (the last
+ * query sees every key).  A query that sees no key, and a token of no cloud, gets
+ * zeros and lse -inf; its gradients are zeros.  A cloud's result depends on
+ * that cloud's tokens alone, whatever its neighbours hold.
+ * dtype: TPO_F32, TPO_F16, TPO_BF16; width 1 to 256.  Strides are in elements, the
+ * width dimension has stride 1.  Sums are fp32; for 16-bit types the probabilities
+ * are rounded to that type before they multiply v (and dS before k and q). */
+typedef struct tpo_packed_attention {
+  int dtype, causal;
+  int64_t clouds, heads, kv_heads, width, tokens_q, tokens_k;
+  const int64_t *offsets_q, *offsets_k;
+  float scale; /* > 0 */
+  const void *q, *k, *v;
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+} tpo_packed_attention;
+/* o (tokens_q, heads, width) of type dtype, lse (heads, tokens_q) fp32: natural
+ * logarithm of the sum of exponentials; lse may be NULL where no backward follows. */
+TPO_API int tpo_packed_attention_fwd(const tpo_packed_attention* p, void* o, float* lse, void* stream);
+/* dq (tokens_q, heads, width), dk, dv (tokens_k, kv_heads, width), contiguous, fully
+ * written, each NULL where it is not wanted (dk and dv together).  No atomics touch
+ * them: every run gives the same bits. */
+TPO_API size_t tpo_packed_attention_bwd_workspace_size(int64_t tokens_q, int64_t heads);
+TPO_API int tpo_packed_attention_bwd(const tpo_packed_attention* p, const void* o, const float* lse,
+                                     const void* grad_o, int64_t grad_o_token_stride,
+                                     int64_t grad_o_head_stride, void* dq, void* dk, void* dv,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention of one token per cloud over a cache: q (N, H, D), k and v (N, P, Hk, D)
+ * with lengths (N) int64 (clamped to [0, P]) -> o (N, H, D) contiguous.  Slots at or
+ * beyond lengths[n] are not read; length 0 gives zeros.  Strides in elements:
+ * q_stride {cloud, head}, k_stride and v_stride {cloud, token, head} (host arrays). */
+TPO_API size_t tpo_cached_attention_workspace_size(int64_t N, int64_t H, int64_t Hk, int64_t P, int64_t D);
+TPO_API int tpo_cached_attention(int dtype, const void* q, const int64_t* q_stride, const void* k,
+                                 const int64_t* k_stride, const void* v, const int64_t* v_stride,
+                                 const int64_t* lengths, int64_t N, int64_t P, int64_t H, int64_t Hk,
+                                 int64_t D, float scale, void* o, void* workspace,
+                                 size_t workspace_bytes, void* stream);
 
 /* Measurement aid (no counterpart in the reference): the sustained issue rate of
  * one arithmetic instruction kind on the current device, for quoting the CUDA-core

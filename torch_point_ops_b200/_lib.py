@@ -21,6 +21,8 @@ torch.ops.load_library(TORCH_BINDING_PATH)
 chamfer_ops = torch.ops.torch_point_ops_b200_chamfer
 knn_ops = torch.ops.torch_point_ops_b200_knn
 fps_ops = torch.ops.torch_point_ops_b200_fps
+norm_ops = torch.ops.torch_point_ops_b200_norm
+attention_ops = torch.ops.torch_point_ops_b200_attention
 
 _capi = None
 

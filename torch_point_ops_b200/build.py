@@ -27,7 +27,8 @@ CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
 CU_SOURCES = ["chamfer_fwd.cu", "chamfer_bwd.cu", "knn.cu", "capi.cu", "chamfer_noalloc.cu", "gather_points.cu", "fps.cu",
-              "pipe_probe.cu"]
+              "pipe_probe.cu", "layer_norm.cu", "attention.cu", "attention_simt.cu", "attention_cached.cu"]
+CPP_SOURCES = ["torch_ops.cpp", "torch_token_ops.cpp"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
@@ -82,14 +83,22 @@ def build(force: bool = False, verbose: bool = False) -> str:
     import torch
     from torch.utils import cpp_extension as ce
 
-    src = os.path.join(CSRC, "torch_ops.cpp")
-    if force or _stale(TORCH_LIB, [src, CAPI_LIB] + hdrs):
-        tdir = os.path.dirname(torch.__file__)
-        inc = [f"-I{p}" for p in ce.include_paths()] + [f"-I{os.path.join(CUDA_HOME, 'include')}",
-                                                        f"-I{sysconfig.get_paths()['include']}"]
-        abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-        _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
-              src, "-o", TORCH_LIB] + inc + [
+    objs = []
+    jobs = []
+    tdir = os.path.dirname(torch.__file__)
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    inc = [f"-I{p}" for p in ce.include_paths()] + [f"-I{os.path.join(CUDA_HOME, 'include')}",
+                                                    f"-I{sysconfig.get_paths()['include']}"]
+    for name in CPP_SOURCES:
+        s = os.path.join(CSRC, name)
+        o = os.path.join(OBJ, name.replace(".cpp", ".cpp.o"))
+        objs.append(o)
+        if force or _stale(o, [s] + glob.glob(os.path.join(ROOT, "include", "*.h"))):
+            jobs.append(["g++", "-O2", "-std=c++17", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-c", s, "-o", o] + inc)
+    with cf.ThreadPoolExecutor(max_workers=max(1, len(jobs))) as ex:
+        list(ex.map(_run, jobs))
+    if force or _stale(TORCH_LIB, objs + [CAPI_LIB]):
+        _run(["g++", "-shared"] + objs + ["-o", TORCH_LIB,
               f"-L{LIB}", "-ltpo_b200", f"-L{os.path.join(tdir, 'lib')}",
               "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
               "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{os.path.join(tdir, 'lib')}"])

@@ -1,0 +1,98 @@
+// Shared by the attention kernels: the problem's description and the map from
+// blocks to tiles of packed clouds.
+#pragma once
+
+#include "tpo_internal.h"
+#include "tpo_types.cuh"
+
+namespace tpo {
+
+// Set by a kernel that met offsets that decrease or leave [0, tokens]
+// (TPO_DEVERR_BAD_OFFSETS); what it reads and writes stays clamped.
+constexpr unsigned kErrBadOffsets = 4u;
+static __device__ unsigned g_attention_error = 0;  // one per translation unit
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// One packed problem, by value to every kernel.  Strides in elements; the width
+// dimension has stride 1.  o, dq are (Tq, H, D), dk, dv (Tk, Hk, D), lse and
+// delta (H, Tq), all contiguous.
+struct PackedArgs {
+  const void *q, *k, *v, *go;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, go_st, go_sh;  // token and head strides
+  const int64_t *off_q, *off_k;
+  void *o, *dq, *dk, *dv;
+  float *lse, *delta;
+  const unsigned* go_max;  // largest |go| as bits of a float (fp16 backward), or null
+  int64_t Tq, Tk;
+  int B, H, Hk, D, causal;
+  float scale;
+};
+
+// A tile of one cloud: rows [row0, row0 + rows) of the packed tensor that was
+// tiled; [a0, a0 + na) and [b0, b0 + nb) are the cloud's rows there and in the
+// other tensor.  rows == 0: nothing to do.
+struct Tile {
+  int64_t row0, a0, b0;
+  int rows;
+  int64_t na, nb;
+};
+
+// Blocks per head for tiles of BM rows: with e(i) the start of cloud i, cloud i
+// gets the slots from e(i)/BM + i on.  The next cloud's first slot is at least
+// ceil(length / BM) further, so every tile has a slot, at most one slot per cloud
+// stays empty, and the host needs no lengths.  Two more "clouds" cover the tokens
+// before the first and after the last offset; nobody attends there.
+inline int64_t packed_slots(int64_t tokens, int64_t clouds, int BM) { return tokens / BM + clouds + 2; }
+
+// All 32 lanes of a warp call this with the same slot.
+__device__ __forceinline__ Tile find_tile(const int64_t* off, int64_t T, const int64_t* other,
+                                          int64_t To, int B, int BM, int64_t slot) {
+  const int lane = threadIdx.x & 31;
+  auto start = [&](int i) -> int64_t {  // clamped start of extended cloud i in [0, B + 2]
+    if (i == 0) return 0;
+    if (i == B + 2) return T;
+    return min64(max64(off[i - 1], 0), T);
+  };
+  // greatest i in [lo, hi) with start(i)/BM + i <= slot; 32 probes a step
+  int lo = 0, hi = B + 2;
+  while (hi - lo > 1) {
+    const int step = (hi - lo + 31) / 32;
+    const int i = lo + lane * step;
+    const bool le = i < hi && (lane == 0 || start(i) / BM + i <= slot);
+    const unsigned m = __ballot_sync(0xffffffffu, le);
+    const int last = 31 - __clz(m);
+    hi = min(hi, lo + (last + 1) * step);
+    lo += last * step;
+  }
+  Tile t;
+  t.a0 = start(lo);
+  const int64_t end = start(lo + 1);
+  t.na = max64(end - t.a0, 0);
+  t.row0 = t.a0 + (slot - (t.a0 / BM + lo)) * BM;
+  t.rows = (int)max64(0, min64(end - t.row0, BM));
+  if (t.row0 < t.a0) t.rows = 0;
+  t.b0 = 0;
+  t.nb = 0;
+  if (lo >= 1 && lo <= B) {
+    const int64_t r0 = other[lo - 1], r1 = other[lo];
+    t.b0 = min64(max64(r0, 0), To);
+    t.nb = max64(min64(max64(r1, 0), To) - t.b0, 0);
+    if (lane == 0 && (r0 < 0 || r1 < r0 || r1 > To || off[lo - 1] < 0 || off[lo] < off[lo - 1] || off[lo] > T))
+      atomicOr(&g_attention_error, kErrBadOffsets);
+  }
+  return t;
+}
+
+inline int read_attention_error(unsigned* out, bool clear) {
+  int s = cuda_status(cudaMemcpyFromSymbol(out, g_attention_error, sizeof(unsigned)));
+  if (s || !clear) return s;
+  const unsigned zero = 0;
+  return cuda_status(cudaMemcpyToSymbol(g_attention_error, &zero, sizeof(unsigned)));
+}
+
+int packed_simt_forward(int dtype, const PackedArgs& a, cudaStream_t st);
+int packed_simt_backward(int dtype, const PackedArgs& a, cudaStream_t st);
+int packed_delta(int dtype, const PackedArgs& a, cudaStream_t st);
+
+}  // namespace tpo

@@ -1,0 +1,443 @@
+// Attention over packed clouds on the FP32 pipe: every dtype, width up to 256,
+// any strides.  Exact fp32 products, so it is the path of fp32 inputs; 16-bit
+// inputs come here only where the tensor-core kernels' alignment or width rules
+// do not hold.
+//
+//   S = scale * Q K^T over the keys that a row sees,  P = softmax(S),  O = P V
+//   dV = P^T dO,  dP = dO V^T,  dS = P * (dP - delta) * scale,  delta = dO . O
+//   dQ = dS K,  dK = dS^T Q (dK and dV summed over the query heads of a group)
+//
+// Forward: one pass over the keys with the running maximum and sum of each row.
+// Backward: P is rebuilt from the forward's log-sum-exp; one kernel owns key
+// tiles (dK, dV), one owns query tiles (dQ), so nothing is added by atomics and
+// every run gives the same bits, at 7 products in place of 5.
+//
+// 256 threads as 16 x 16; a thread holds RM rows (ty) x CN columns (tx + 16 c) of
+// a score tile and RM rows x DP/16 columns of an output tile.  Both products read
+// four elements of the summed dimension per 16-byte shared-memory load: rows are
+// broadcast, columns sit in rows of DP + 4 floats (two wavefronts per load, no
+// bank conflicts), which gives 32 FMA cycles per 16 load cycles at RM = 8.
+#include "attention_common.cuh"
+
+namespace tpo {
+namespace {
+
+constexpr int kThreads = 256;
+
+// rows x DP tile from packed memory into fp32 shared memory (row pitch DP + 4);
+// rows beyond `valid` and columns beyond D are zero, so that nothing from another
+// cloud (a NaN would survive 0 * NaN) enters a product.
+template <typename T, int VEC, int DP>
+__device__ __forceinline__ void load_tile(float* dst, const T* src, int64_t stride, int rows,
+                                          int valid, int D) {
+  constexpr int PER_ROW = DP / VEC;
+  for (int i = threadIdx.x; i < rows * PER_ROW; i += kThreads) {
+    const int r = i / PER_ROW, c = (i % PER_ROW) * VEC;
+    float v[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = 0.f;
+    if (r < valid && c < D) load_vec<VEC>(src + r * stride + c, v);
+    float* d = dst + r * (DP + 4) + c;
+    if (VEC % 4 == 0) {
+#pragma unroll
+      for (int j = 0; j < VEC; j += 4)
+        *reinterpret_cast<float4*>(d + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) d[j] = v[j];
+    }
+  }
+}
+
+// s[r][c] = sum_d a[ty*RM + r][d] * b[tx + 16c][d]
+template <int DP, int RM, int CN>
+__device__ __forceinline__ void product_nt(float (&s)[RM][CN], const float* a, const float* b, int ty,
+                                           int tx) {
+#pragma unroll
+  for (int r = 0; r < RM; ++r)
+#pragma unroll
+    for (int c = 0; c < CN; ++c) s[r][c] = 0.f;
+  const float* ar = a + ty * RM * (DP + 4);
+  const float* br = b + tx * (DP + 4);
+#pragma unroll 2
+  for (int d = 0; d < DP; d += 4) {
+    float4 bv[CN];
+#pragma unroll
+    for (int c = 0; c < CN; ++c) bv[c] = *reinterpret_cast<const float4*>(br + c * 16 * (DP + 4) + d);
+#pragma unroll
+    for (int r = 0; r < RM; ++r) {
+      const float4 av = *reinterpret_cast<const float4*>(ar + r * (DP + 4) + d);
+#pragma unroll
+      for (int c = 0; c < CN; ++c) {
+        s[r][c] = fmaf(av.x, bv[c].x, s[r][c]);
+        s[r][c] = fmaf(av.y, bv[c].y, s[r][c]);
+        s[r][c] = fmaf(av.z, bv[c].z, s[r][c]);
+        s[r][c] = fmaf(av.w, bv[c].w, s[r][c]);
+      }
+    }
+  }
+}
+
+// o[r][4g + i] += sum_j p[ty*RM + r][j] * v[j][tx*4 + 64g + i]
+template <int DP, int RM, int BN>
+__device__ __forceinline__ void product_nn(float (&o)[RM][DP / 16], const float* p, const float* v,
+                                           int ty, int tx) {
+  const float* pr = p + ty * RM * (BN + 4);
+#pragma unroll 1
+  for (int j = 0; j < BN; j += 4) {
+    float4 pv[RM];
+#pragma unroll
+    for (int r = 0; r < RM; ++r) pv[r] = *reinterpret_cast<const float4*>(pr + r * (BN + 4) + j);
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj) {
+#pragma unroll
+      for (int g = 0; g < DP / 64; ++g) {
+        const float4 vv = *reinterpret_cast<const float4*>(v + (j + jj) * (DP + 4) + tx * 4 + g * 64);
+#pragma unroll
+        for (int r = 0; r < RM; ++r) {
+          const float w = jj == 0 ? pv[r].x : jj == 1 ? pv[r].y : jj == 2 ? pv[r].z : pv[r].w;
+          o[r][g * 4 + 0] = fmaf(w, vv.x, o[r][g * 4 + 0]);
+          o[r][g * 4 + 1] = fmaf(w, vv.y, o[r][g * 4 + 1]);
+          o[r][g * 4 + 2] = fmaf(w, vv.z, o[r][g * 4 + 2]);
+          o[r][g * 4 + 3] = fmaf(w, vv.w, o[r][g * 4 + 3]);
+        }
+      }
+    }
+  }
+}
+
+template <int DP, int RM>
+struct FwdShape {
+  static constexpr int BM = 16 * RM, BN = 64;
+  static constexpr int smem = ((BM + BN) * (DP + 4) + BM * (BN + 4)) * 4;
+};
+
+template <typename T, int VEC, int DP, int RM>
+__global__ void __launch_bounds__(kThreads) packed_simt_fwd_kernel(const PackedArgs a) {
+  using Sh = FwdShape<DP, RM>;
+  constexpr int BM = Sh::BM, BN = Sh::BN, CN = 4;
+  extern __shared__ float4 smem4[];
+  float* qs = reinterpret_cast<float*>(smem4);
+  float* kv = qs + BM * (DP + 4);
+  float* ps = kv + BN * (DP + 4);
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  const int head = blockIdx.y, kvh = head / (a.H / a.Hk);
+  // causal rows late in a cloud see most keys: those blocks start first
+  const int64_t slot = a.causal ? (int64_t)gridDim.x - 1 - blockIdx.x : blockIdx.x;
+  const Tile t = find_tile(a.off_q, a.Tq, a.off_k, a.Tk, a.B, BM, slot);
+  if (t.rows <= 0) return;
+  const int64_t shift = t.nb - t.na;            // a row sees keys up to its place + shift
+  const int64_t first = t.row0 - t.a0;          // place of the tile's first row in its cloud
+  int64_t nk = t.nb;
+  if (a.causal) nk = min64(nk, max64(first + t.rows + shift, 0));
+  const float qscale = a.scale * kLog2e;
+
+  load_tile<T, VEC, DP>(qs, (const T*)a.q + t.row0 * a.q_st + head * a.q_sh, a.q_st, BM, t.rows, a.D);
+  const T* kp = (const T*)a.k + t.b0 * a.k_st + kvh * a.k_sh;
+  const T* vp = (const T*)a.v + t.b0 * a.v_st + kvh * a.v_sh;
+  float o[RM][DP / 16], m[RM], l[RM];
+#pragma unroll
+  for (int r = 0; r < RM; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) o[r][c] = 0.f;
+  }
+  for (int64_t j0 = 0; j0 < nk; j0 += BN) {
+    const int valid = (int)min64(nk - j0, BN);
+    __syncthreads();
+    load_tile<T, VEC, DP>(kv, kp + j0 * a.k_st, a.k_st, BN, valid, a.D);
+    __syncthreads();
+    float s[RM][CN];
+    product_nt<DP, RM, CN>(s, qs, kv, ty, tx);
+    __syncthreads();
+    load_tile<T, VEC, DP>(kv, vp + j0 * a.v_st, a.v_st, BN, valid, a.D);
+#pragma unroll
+    for (int r = 0; r < RM; ++r) {
+      int64_t lim = valid;
+      if (a.causal) lim = min64(lim, first + ty * RM + r + shift + 1 - j0);
+      float mx = m[r];
+#pragma unroll
+      for (int c = 0; c < CN; ++c) {
+        s[r][c] = tx + 16 * c < lim ? s[r][c] * qscale : -INFINITY;
+        mx = fmaxf(mx, s[r][c]);
+      }
+#pragma unroll
+      for (int x = 8; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      const float base = mx == -INFINITY ? 0.f : mx;  // a row that has seen nothing yet
+      const float corr = exp2f(m[r] - base);
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < CN; ++c) {
+        const float p = exp2f(s[r][c] - base);
+        sum += p;
+        ps[(ty * RM + r) * (BN + 4) + tx + 16 * c] = p;
+      }
+      m[r] = mx;
+      l[r] = l[r] * corr + sum;
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) o[r][c] *= corr;
+    }
+    __syncthreads();
+    product_nn<DP, RM, BN>(o, ps, kv, ty, tx);
+  }
+#pragma unroll
+  for (int r = 0; r < RM; ++r) {
+    float sum = l[r];
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    const int row = ty * RM + r;
+    if (row >= t.rows) continue;
+    const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // NaN stays NaN
+    const int64_t tok = t.row0 + row;
+    if (tx == 0 && a.lse) a.lse[(int64_t)head * a.Tq + tok] = sum == 0.f ? -INFINITY : (m[r] + log2f(sum)) * kLn2;
+    T* op = (T*)a.o + (tok * a.H + head) * a.D;
+#pragma unroll
+    for (int g = 0; g < DP / 64; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = tx * 4 + g * 64 + i;
+        if (c < a.D) op[c] = from_acc<T>(o[r][g * 4 + i] * inv);
+      }
+  }
+}
+
+// Backward.  DKV: rows are keys (X1 = K, X2 = V), columns queries (Y1 = Q,
+// Y2 = dO), summed over the group's query heads; else rows are queries and
+// columns keys.  In both, s = X1 Y1^T and dp = X2 Y2^T.
+template <int DP, int RM>
+struct BwdShape {
+  static constexpr int BM = 16 * RM, BN = 16 * RM, CN = RM;
+  static constexpr int smem = (2 * (BM + BN) * (DP + 4) + 2 * BM * (BN + 4)) * 4 + 2 * BN * 4;
+};
+
+template <typename T, int VEC, int DP, int RM, bool DKV>
+__global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedArgs a) {
+  using Sh = BwdShape<DP, RM>;
+  constexpr int BM = Sh::BM, BN = Sh::BN, CN = Sh::CN, LD = DP + 4;
+  extern __shared__ float4 smem4[];
+  float* x1 = reinterpret_cast<float*>(smem4);
+  float* x2 = x1 + BM * LD;
+  float* y1 = x2 + BM * LD;
+  float* y2 = y1 + BN * LD;
+  float* ps = y2 + BN * LD;            // P^T (DKV only)
+  float* ds = ps + BM * (BN + 4);      // dS or dS^T
+  float* cl = ds + BM * (BN + 4);      // log-sum-exp and delta of the columns (DKV)
+  float* cd = cl + BN;
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  const int group = a.H / a.Hk;
+  const int64_t slot = !DKV && a.causal ? (int64_t)gridDim.x - 1 - blockIdx.x : blockIdx.x;
+  const Tile t = DKV ? find_tile(a.off_k, a.Tk, a.off_q, a.Tq, a.B, BM, slot)
+                     : find_tile(a.off_q, a.Tq, a.off_k, a.Tk, a.B, BM, slot);
+  if (t.rows <= 0) return;
+  const int64_t nq = DKV ? t.nb : t.na, nkeys = DKV ? t.na : t.nb, shift = nkeys - nq;
+  const int64_t first = t.row0 - t.a0;
+  // columns that any row of the tile meets
+  int64_t c_begin = 0, c_end = t.nb;
+  if (a.causal) {
+    if (DKV) c_begin = max64(0, first - shift) / BN * BN;
+    else c_end = min64(c_end, max64(first + t.rows + shift, 0));
+  }
+  const float qscale = a.scale * kLog2e;
+  const int kvh = DKV ? blockIdx.y : blockIdx.y / group;
+  const int head0 = DKV ? kvh * group : blockIdx.y, heads = DKV ? group : 1;
+  const T* kp = (const T*)a.k + kvh * a.k_sh;
+  const T* vp = (const T*)a.v + kvh * a.v_sh;
+  float acc1[RM][DP / 16], acc2[DKV ? RM : 1][DKV ? DP / 16 : 1];
+#pragma unroll
+  for (int r = 0; r < RM; ++r)
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) {
+      acc1[r][c] = 0.f;
+      if (DKV) acc2[r][c] = 0.f;
+    }
+  float row_lse[RM], row_delta[RM];
+  if (DKV) {
+    load_tile<T, VEC, DP>(x1, kp + t.row0 * a.k_st, a.k_st, BM, t.rows, a.D);
+    load_tile<T, VEC, DP>(x2, vp + t.row0 * a.v_st, a.v_st, BM, t.rows, a.D);
+  } else {
+    load_tile<T, VEC, DP>(x1, (const T*)a.q + t.row0 * a.q_st + head0 * a.q_sh, a.q_st, BM, t.rows, a.D);
+    load_tile<T, VEC, DP>(x2, (const T*)a.go + t.row0 * a.go_st + head0 * a.go_sh, a.go_st, BM, t.rows, a.D);
+#pragma unroll
+    for (int r = 0; r < RM; ++r) {
+      const int row = ty * RM + r;
+      const bool in = row < t.rows;
+      row_lse[r] = in ? a.lse[(int64_t)head0 * a.Tq + t.row0 + row] * kLog2e : 0.f;
+      row_delta[r] = in ? a.delta[(int64_t)head0 * a.Tq + t.row0 + row] : 0.f;
+    }
+  }
+  for (int h = 0; h < heads; ++h) {
+    const int head = head0 + h;
+    for (int64_t c0 = c_begin; c0 < c_end; c0 += BN) {
+      const int valid = (int)min64(c_end - c0, BN);
+      __syncthreads();
+      if (DKV) {
+        const int64_t tok = t.b0 + c0;
+        load_tile<T, VEC, DP>(y1, (const T*)a.q + tok * a.q_st + head * a.q_sh, a.q_st, BN, valid, a.D);
+        load_tile<T, VEC, DP>(y2, (const T*)a.go + tok * a.go_st + head * a.go_sh, a.go_st, BN, valid, a.D);
+        if (threadIdx.x < BN) {
+          const bool in = threadIdx.x < valid;
+          cl[threadIdx.x] = in ? a.lse[(int64_t)head * a.Tq + tok + threadIdx.x] * kLog2e : 0.f;
+          cd[threadIdx.x] = in ? a.delta[(int64_t)head * a.Tq + tok + threadIdx.x] : 0.f;
+        }
+      } else {
+        load_tile<T, VEC, DP>(y1, kp + (t.b0 + c0) * a.k_st, a.k_st, BN, valid, a.D);
+        load_tile<T, VEC, DP>(y2, vp + (t.b0 + c0) * a.v_st, a.v_st, BN, valid, a.D);
+      }
+      __syncthreads();
+      float s[RM][CN], dp[RM][CN];
+      product_nt<DP, RM, CN>(s, x1, y1, ty, tx);
+      product_nt<DP, RM, CN>(dp, x2, y2, ty, tx);
+#pragma unroll
+      for (int r = 0; r < RM; ++r) {
+        const int row = ty * RM + r;
+        int64_t lo = 0, hi = row < t.rows ? valid : 0;  // columns that this row meets
+        if (a.causal) {
+          if (DKV) lo = first + row - shift - c0;       // queries from the key's place - shift on
+          else hi = min64(hi, first + row + shift + 1 - c0);
+        }
+#pragma unroll
+        for (int c = 0; c < CN; ++c) {
+          const int col = tx + 16 * c;
+          const float lse = DKV ? cl[col] : row_lse[r], delta = DKV ? cd[col] : row_delta[r];
+          const bool in = col >= lo && col < hi;
+          const float p = in ? exp2f(fmaf(s[r][c], qscale, -lse)) : 0.f;
+          if (DKV) ps[row * (BN + 4) + col] = p;
+          ds[row * (BN + 4) + col] = in ? p * (dp[r][c] - delta) : 0.f;
+        }
+      }
+      __syncthreads();
+      product_nn<DP, RM, BN>(acc1, ds, y1, ty, tx);
+      if constexpr (DKV) product_nn<DP, RM, BN>(acc2, ps, y2, ty, tx);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < RM; ++r) {
+    const int row = ty * RM + r;
+    if (row >= t.rows) continue;
+    const int64_t at = DKV ? ((t.row0 + row) * a.Hk + kvh) * a.D : ((t.row0 + row) * a.H + head0) * a.D;
+    T* d1 = (T*)(DKV ? a.dk : a.dq) + at;
+    T* d2 = DKV ? (T*)a.dv + at : nullptr;
+#pragma unroll
+    for (int g = 0; g < DP / 64; ++g)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = tx * 4 + g * 64 + i;
+        if (c < a.D) {
+          d1[c] = from_acc<T>(acc1[r][g * 4 + i] * a.scale);
+          if (DKV) d2[c] = from_acc<T>(acc2[r][g * 4 + i]);
+        }
+      }
+  }
+}
+
+// delta = dO . O per (head, token): a warp per row.
+template <typename T>
+__global__ void __launch_bounds__(256) packed_delta_kernel(const PackedArgs a) {
+  const int64_t rows = a.Tq * a.H;
+  const int lane = threadIdx.x & 31;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += (int64_t)gridDim.x * 8) {
+    const int64_t tok = r / a.H;
+    const int head = (int)(r - tok * a.H);
+    const T* o = (const T*)a.o + r * a.D;
+    const T* g = (const T*)a.go + tok * a.go_st + head * a.go_sh;
+    float s = 0.f;
+    for (int c = lane; c < a.D; c += 32) s += to_acc(o[c]) * to_acc(g[c]);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+    if (lane == 0) a.delta[(int64_t)head * a.Tq + tok] = s;
+  }
+}
+
+template <typename K>
+int set_smem(K kern, int bytes) {
+  return cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+}
+
+template <typename T, int VEC, int DP, int RM>
+int fwd(const PackedArgs& a, cudaStream_t st) {
+  using Sh = FwdShape<DP, RM>;
+  auto kern = packed_simt_fwd_kernel<T, VEC, DP, RM>;
+  int s = set_smem(kern, Sh::smem);
+  if (s) return s;
+  kern<<<dim3((unsigned)packed_slots(a.Tq, a.B, Sh::BM), a.H), kThreads, Sh::smem, st>>>(a);
+  return check_launch();
+}
+
+template <typename T, int VEC, int DP, int RM>
+int bwd(const PackedArgs& a, cudaStream_t st) {
+  using Sh = BwdShape<DP, RM>;
+  if (a.dk && a.Tk > 0) {
+    auto kern = packed_simt_bwd_kernel<T, VEC, DP, RM, true>;
+    int s = set_smem(kern, Sh::smem);
+    if (s) return s;
+    kern<<<dim3((unsigned)packed_slots(a.Tk, a.B, Sh::BM), a.Hk), kThreads, Sh::smem, st>>>(a);
+    if ((s = check_launch())) return s;
+  }
+  if (a.dq && a.Tq > 0) {
+    auto kern = packed_simt_bwd_kernel<T, VEC, DP, RM, false>;
+    int s = set_smem(kern, Sh::smem);
+    if (s) return s;
+    kern<<<dim3((unsigned)packed_slots(a.Tq, a.B, Sh::BM), a.H), kThreads, Sh::smem, st>>>(a);
+    if ((s = check_launch())) return s;
+  }
+  return TPO_OK;
+}
+
+// 16-byte loads where every row of every input starts on 16 bytes and the width
+// is whole vectors.
+template <typename T>
+bool vec_ok(const PackedArgs& a, bool backward) {
+  constexpr int V = 16 / sizeof(T);
+  auto ok = [](const void* p, int64_t s1, int64_t s2) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s1 % V == 0 && s2 % V == 0;
+  };
+  return a.D % V == 0 && ok(a.q, a.q_st, a.q_sh) && ok(a.k, a.k_st, a.k_sh) && ok(a.v, a.v_st, a.v_sh) &&
+         (!backward || ok(a.go, a.go_st, a.go_sh));
+}
+
+template <typename T, int VEC>
+int fwd_width(const PackedArgs& a, cudaStream_t st) {
+  if (a.D <= 64) return fwd<T, VEC, 64, 8>(a, st);
+  if (a.D <= 128) return fwd<T, VEC, 128, 4>(a, st);
+  return fwd<T, VEC, 256, 4>(a, st);
+}
+template <typename T, int VEC>
+int bwd_width(const PackedArgs& a, cudaStream_t st) {
+  if (a.D <= 64) return bwd<T, VEC, 64, 4>(a, st);
+  if (a.D <= 128) return bwd<T, VEC, 128, 4>(a, st);
+  return bwd<T, VEC, 256, 2>(a, st);
+}
+
+template <typename T>
+int fwd_typed(const PackedArgs& a, cudaStream_t st) {
+  return vec_ok<T>(a, false) ? fwd_width<T, 16 / sizeof(T)>(a, st) : fwd_width<T, 1>(a, st);
+}
+template <typename T>
+int bwd_typed(const PackedArgs& a, cudaStream_t st) {
+  return vec_ok<T>(a, true) ? bwd_width<T, 16 / sizeof(T)>(a, st) : bwd_width<T, 1>(a, st);
+}
+
+template <typename T>
+int delta_typed(const PackedArgs& a, cudaStream_t st) {
+  packed_delta_kernel<T><<<(unsigned)min64((a.Tq * a.H + 7) / 8, 148 * 32), 256, 0, st>>>(a);
+  return check_launch();
+}
+
+}  // namespace
+
+#define TPO_DISPATCH(F)                                              \
+  switch (dtype) {                                                   \
+    case TPO_F32: return F<float>(a, st);                            \
+    case TPO_F16: return F<__half>(a, st);                           \
+    case TPO_BF16: return F<__nv_bfloat16>(a, st);                   \
+    default: return set_error(TPO_ERR_INVALID_ARGUMENT, "packed_attention: dtype must be f32, f16 or bf16"); \
+  }
+
+int packed_simt_forward(int dtype, const PackedArgs& a, cudaStream_t st) { TPO_DISPATCH(fwd_typed) }
+int packed_simt_backward(int dtype, const PackedArgs& a, cudaStream_t st) { TPO_DISPATCH(bwd_typed) }
+int packed_delta(int dtype, const PackedArgs& a, cudaStream_t st) { TPO_DISPATCH(delta_typed) }
+
+int attention_simt_error_flags(unsigned* out, bool clear) { return read_attention_error(out, clear); }
+
+}  // namespace tpo

@@ -49,11 +49,12 @@ const char* tpo_status_string(int status) {
 
 int tpo_device_error_flags(unsigned* flags, int clear) {
   if (!flags) return fail(TPO_ERR_INVALID_ARGUMENT, "device_error_flags: null output");
-  unsigned a = 0, b = 0, c = 0;
+  unsigned a = 0, b = 0, c = 0, d = 0;
   int s = device_error_flags(&a, clear != 0);
   if (!s) s = fps_device_error_flags(&b, clear != 0);
   if (!s) s = knn_device_error_flags(&c, clear != 0);
-  *flags = a | b | c;
+  if (!s) s = attention_simt_error_flags(&d, clear != 0);
+  *flags = a | b | c | d;
   return s;
 }
 
@@ -397,6 +398,150 @@ int tpo_gather_points_bwd(int dtype, const void* grad_out, const int64_t* idx, i
       (s = cuda_status(cudaMemsetAsync(grad_points, 0, (size_t)dtype_size(dtype) * N * C * P, st))))
     return s;
   return gather_points_backward(dtype, grad_out, idx, N, C, P, M, grad_points, st);
+}
+
+// ---- token operators: layer norm, attention ----
+
+static int check_layer_norm(int dtype, int wdtype, const void* x, int64_t x_stride, int64_t rows,
+                            int64_t width) {
+  const bool half = dtype == TPO_F16 || dtype == TPO_BF16;
+  if (dtype < TPO_F32 || dtype > TPO_BF16)
+    return fail(TPO_ERR_INVALID_ARGUMENT, "layer_norm: dtype must be f32, f16, bf16 or f64");
+  if (wdtype != dtype && !(half && wdtype == TPO_F32))
+    return fail(TPO_ERR_INVALID_ARGUMENT, "layer_norm: weight and bias must have the rows' dtype, or f32 with 16-bit rows");
+  if (rows < 0 || width < 0 || width > INT32_MAX)
+    return fail(TPO_ERR_INVALID_ARGUMENT, "layer_norm: bad shape");
+  if (x_stride < 0) return fail(TPO_ERR_INVALID_ARGUMENT, "layer_norm: negative row stride");
+  if (rows * width > 0 && !x) return fail(TPO_ERR_INVALID_ARGUMENT, "layer_norm: null input");
+  return TPO_OK;
+}
+
+int tpo_layer_norm_fwd(int dtype, int wdtype, const void* x, int64_t x_stride, const void* weight,
+                       const void* bias, int64_t rows, int64_t width, double eps, void* y, void* mean,
+                       void* rstd, void* stream) {
+  int s = check_layer_norm(dtype, wdtype, x, x_stride, rows, width);
+  if (s) return s;
+  if (!(eps >= 0)) return fail(TPO_ERR_INVALID_ARGUMENT, "layer_norm: eps must not be negative");
+  if (!mean != !rstd) return fail(TPO_ERR_INVALID_ARGUMENT, "layer_norm: mean and rstd go together");
+  if (rows == 0 || width == 0) return TPO_OK;
+  if (!y) return fail(TPO_ERR_INVALID_ARGUMENT, "layer_norm: null output");
+  return layer_norm_forward(dtype, wdtype, x, x_stride, weight, bias, rows, width, eps, y, mean, rstd,
+                            (cudaStream_t)stream);
+}
+
+size_t tpo_layer_norm_bwd_workspace_size(int dtype, int64_t rows, int64_t width) {
+  if (dtype < TPO_F32 || dtype > TPO_BF16 || rows <= 0 || width <= 0) return 0;
+  return layer_norm_bwd_workspace_size(dtype, rows, width);
+}
+
+int tpo_layer_norm_bwd(int dtype, int wdtype, const void* x, int64_t x_stride, const void* dy,
+                       int64_t dy_stride, const void* weight, const void* mean, const void* rstd,
+                       int64_t rows, int64_t width, void* dx, void* dweight, void* dbias,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+  int s = check_layer_norm(dtype, wdtype, x, x_stride, rows, width);
+  if (s) return s;
+  if (dy_stride < 0) return fail(TPO_ERR_INVALID_ARGUMENT, "layer_norm_bwd: negative row stride");
+  if (width == 0) return TPO_OK;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (rows == 0) {  // sums over no rows
+    const size_t n = (size_t)dtype_size(wdtype) * width;
+    if (dweight && (s = cuda_status(cudaMemsetAsync(dweight, 0, n, st)))) return s;
+    return dbias ? cuda_status(cudaMemsetAsync(dbias, 0, n, st)) : TPO_OK;
+  }
+  if (!dy || !mean || !rstd) return fail(TPO_ERR_INVALID_ARGUMENT, "layer_norm_bwd: null pointer");
+  if (!dx && !dweight && !dbias) return TPO_OK;
+  if ((dweight || dbias) &&
+      (!workspace || workspace_bytes < layer_norm_bwd_workspace_size(dtype, rows, width)))
+    return fail(TPO_ERR_WORKSPACE, "layer_norm_bwd: workspace missing or smaller than tpo_layer_norm_bwd_workspace_size()");
+  if ((uintptr_t)workspace % 16) return fail(TPO_ERR_WORKSPACE, "layer_norm_bwd: workspace must be 16-byte aligned");
+  return layer_norm_backward(dtype, wdtype, x, x_stride, dy, dy_stride, weight, mean, rstd, rows, width,
+                             dx, dweight, dbias, workspace, st);
+}
+
+static bool attention_dtype(int dt) { return dt == TPO_F32 || dt == TPO_F16 || dt == TPO_BF16; }
+
+static int check_packed(const tpo_packed_attention* p) {
+  if (!p) return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention: null problem");
+  if (!attention_dtype(p->dtype)) return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention: dtype must be f32, f16 or bf16");
+  if (p->clouds < 0 || p->clouds > (1 << 24) || p->tokens_q < 0 || p->tokens_k < 0 ||
+      p->tokens_q >= (int64_t(1) << 31) || p->tokens_k >= (int64_t(1) << 31))
+    return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention: bad shape");
+  if (p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads != 0 || p->heads > 65535)
+    return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention: heads must be a multiple of kv_heads (at most 65535)");
+  if (p->width < 1) return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention: width must be positive");
+  if (p->width > kAttentionMaxWidth) return fail(TPO_ERR_UNSUPPORTED, "packed_attention: width is limited to 256");
+  if (!(p->scale > 0) || p->scale > 1e30f)
+    return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention: scale must be positive and finite");
+  if (p->q_token_stride < 0 || p->q_head_stride < 0 || p->k_token_stride < 0 || p->k_head_stride < 0 ||
+      p->v_token_stride < 0 || p->v_head_stride < 0)
+    return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention: negative stride");
+  if (!p->offsets_q || !p->offsets_k) return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention: null offsets");
+  if ((p->tokens_q > 0 && !p->q) || (p->tokens_k > 0 && (!p->k || !p->v)))
+    return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention: null input");
+  return TPO_OK;
+}
+
+int tpo_packed_attention_fwd(const tpo_packed_attention* p, void* o, float* lse, void* stream) {
+  int s = check_packed(p);
+  if (s) return s;
+  if (p->tokens_q == 0) return TPO_OK;
+  if (!o) return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention: null output");
+  return packed_forward(p, o, lse, (cudaStream_t)stream);
+}
+
+size_t tpo_packed_attention_bwd_workspace_size(int64_t tokens_q, int64_t heads) {
+  if (tokens_q < 0 || heads < 0) return 0;
+  return packed_bwd_workspace_size(tokens_q, heads);
+}
+
+int tpo_packed_attention_bwd(const tpo_packed_attention* p, const void* o, const float* lse,
+                             const void* grad_o, int64_t grad_o_token_stride,
+                             int64_t grad_o_head_stride, void* dq, void* dk, void* dv, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+  int s = check_packed(p);
+  if (s) return s;
+  if (!dk != !dv) return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention_bwd: dk and dv go together");
+  if (grad_o_token_stride < 0 || grad_o_head_stride < 0)
+    return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention_bwd: negative stride");
+  if (p->tokens_q > 0 && (!o || !lse || !grad_o))
+    return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention_bwd: null pointer");
+  if (workspace_bytes < packed_bwd_workspace_size(p->tokens_q, p->heads) || !workspace)
+    return fail(TPO_ERR_WORKSPACE, "packed_attention_bwd: workspace missing or smaller than tpo_packed_attention_bwd_workspace_size()");
+  if ((uintptr_t)workspace % 256) return fail(TPO_ERR_WORKSPACE, "packed_attention_bwd: workspace must be 256-byte aligned");
+  return packed_backward(p, o, lse, grad_o, grad_o_token_stride, grad_o_head_stride, dq, dk, dv,
+                         workspace, (cudaStream_t)stream);
+}
+
+size_t tpo_cached_attention_workspace_size(int64_t N, int64_t H, int64_t Hk, int64_t P, int64_t D) {
+  if (N <= 0 || H <= 0 || Hk <= 0 || P < 0 || D <= 0) return 0;
+  return cached_workspace_size(N, H, Hk, P, D);
+}
+
+int tpo_cached_attention(int dtype, const void* q, const int64_t* q_stride, const void* k,
+                         const int64_t* k_stride, const void* v, const int64_t* v_stride,
+                         const int64_t* lengths, int64_t N, int64_t P, int64_t H, int64_t Hk, int64_t D,
+                         float scale, void* o, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!attention_dtype(dtype)) return fail(TPO_ERR_INVALID_ARGUMENT, "cached_attention: dtype must be f32, f16 or bf16");
+  if (N < 0 || N > 65535 || P < 0 || P >= (int64_t(1) << 31))
+    return fail(TPO_ERR_INVALID_ARGUMENT, "cached_attention: bad shape (at most 65535 clouds)");
+  if (H < 1 || Hk < 1 || H % Hk != 0 || H > 65535)
+    return fail(TPO_ERR_INVALID_ARGUMENT, "cached_attention: heads must be a multiple of kv_heads (at most 65535)");
+  if (D < 1) return fail(TPO_ERR_INVALID_ARGUMENT, "cached_attention: width must be positive");
+  if (D > kAttentionMaxWidth) return fail(TPO_ERR_UNSUPPORTED, "cached_attention: width is limited to 256");
+  if (!(scale > 0) || scale > 1e30f)
+    return fail(TPO_ERR_INVALID_ARGUMENT, "cached_attention: scale must be positive and finite");
+  if (N == 0) return TPO_OK;
+  if (!q_stride || !k_stride || !v_stride) return fail(TPO_ERR_INVALID_ARGUMENT, "cached_attention: null strides");
+  for (int i = 0; i < 3; ++i)
+    if ((i < 2 && q_stride[i] < 0) || k_stride[i] < 0 || v_stride[i] < 0)
+      return fail(TPO_ERR_INVALID_ARGUMENT, "cached_attention: negative stride");
+  if (!q || !o || !lengths || (P > 0 && (!k || !v))) return fail(TPO_ERR_INVALID_ARGUMENT, "cached_attention: null pointer");
+  const size_t need = cached_workspace_size(N, H, Hk, P, D);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(TPO_ERR_WORKSPACE, "cached_attention: workspace missing or smaller than tpo_cached_attention_workspace_size()");
+  if ((uintptr_t)workspace % 16) return fail(TPO_ERR_WORKSPACE, "cached_attention: workspace must be 16-byte aligned");
+  return cached_attention(dtype, q, q_stride, k, k_stride, v, v_stride, lengths, N, P, H, Hk, D, scale, o,
+                          workspace, (cudaStream_t)stream);
 }
 
 }  // extern "C"

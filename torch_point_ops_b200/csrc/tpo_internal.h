@@ -80,6 +80,27 @@ int gather_points_forward(int dtype, const void* pts, const int64_t* idx, int64_
 int gather_points_backward(int dtype, const void* gout, const int64_t* idx, int64_t N, int64_t C,
                            int64_t P, int64_t M, void* gpts, cudaStream_t st);
 
+size_t layer_norm_bwd_workspace_size(int dtype, int64_t rows, int64_t width);
+int layer_norm_forward(int dtype, int wdtype, const void* x, int64_t x_stride, const void* weight,
+                       const void* bias, int64_t rows, int64_t width, double eps, void* y, void* mean,
+                       void* rstd, cudaStream_t st);
+int layer_norm_backward(int dtype, int wdtype, const void* x, int64_t x_stride, const void* dy,
+                        int64_t dy_stride, const void* weight, const void* mean, const void* rstd,
+                        int64_t rows, int64_t width, void* dx, void* dweight, void* dbias, void* ws,
+                        cudaStream_t st);
+constexpr int64_t kAttentionMaxWidth = 256;
+size_t packed_bwd_workspace_size(int64_t tokens_q, int64_t heads);
+int packed_forward(const tpo_packed_attention* p, void* o, float* lse, cudaStream_t st);
+int packed_backward(const tpo_packed_attention* p, const void* o, const float* lse, const void* grad_o,
+                    int64_t go_token_stride, int64_t go_head_stride, void* dq, void* dk, void* dv,
+                    void* ws, cudaStream_t st);
+size_t cached_workspace_size(int64_t N, int64_t H, int64_t Hk, int64_t P, int64_t D);
+int cached_attention(int dtype, const void* q, const int64_t* q_stride, const void* k,
+                     const int64_t* k_stride, const void* v, const int64_t* v_stride,
+                     const int64_t* lengths, int64_t N, int64_t P, int64_t H, int64_t Hk, int64_t D,
+                     float scale, void* o, void* ws, cudaStream_t st);
+int attention_simt_error_flags(unsigned* out, bool clear);
+
 // Launches `kern` with programmatic stream serialisation allowed (see pdl_wait).
 template <typename... KArgs, typename... Args>
 inline int launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
@@ -98,7 +119,7 @@ inline int launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem
 }
 
 inline int dtype_size(int dtype) {
-  return dtype == TPO_F32 ? 4 : dtype == TPO_F16 ? 2 : dtype == TPO_F64 ? 8 : 0;
+  return dtype == TPO_F32 ? 4 : dtype == TPO_F16 || dtype == TPO_BF16 ? 2 : dtype == TPO_F64 ? 8 : 0;
 }
 
 }  // namespace tpo

@@ -27,7 +27,7 @@ CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 
 CU_SOURCES = ["chamfer_fwd.cu", "chamfer_bwd.cu", "knn.cu", "capi.cu", "chamfer_noalloc.cu", "gather_points.cu", "fps.cu",
-              "pipe_probe.cu", "layer_norm.cu", "attention.cu", "attention_simt.cu", "attention_cached.cu"]
+              "pipe_probe.cu", "layer_norm.cu", "attention.cu", "attention_simt.cu", "attention_mma.cu", "attention_cached.cu"]
 CPP_SOURCES = ["torch_ops.cpp", "torch_token_ops.cpp"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -30,7 +30,8 @@ size_t packed_bwd_workspace_size(int64_t tokens_q, int64_t heads) {
 int packed_forward(const tpo_packed_attention* p, void* o, float* lse, cudaStream_t st) {
   PackedArgs a = args_of(p);
   a.o = o, a.lse = lse;
-  return packed_simt_forward(p->dtype, a, st);
+  return packed_mma_takes(p->dtype, a, false) ? packed_mma_forward(p->dtype, a, st)
+                                              : packed_simt_forward(p->dtype, a, st);
 }
 
 int packed_backward(const tpo_packed_attention* p, const void* o, const float* lse, const void* grad_o,

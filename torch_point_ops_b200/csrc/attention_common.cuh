@@ -93,6 +93,9 @@ inline int read_attention_error(unsigned* out, bool clear) {
 
 int packed_simt_forward(int dtype, const PackedArgs& a, cudaStream_t st);
 int packed_simt_backward(int dtype, const PackedArgs& a, cudaStream_t st);
+// Whether the tensor-core kernels take the problem, and those kernels.
+bool packed_mma_takes(int dtype, const PackedArgs& a, bool backward);
+int packed_mma_forward(int dtype, const PackedArgs& a, cudaStream_t st);
 int packed_delta(int dtype, const PackedArgs& a, cudaStream_t st);
 
 }  // namespace tpo

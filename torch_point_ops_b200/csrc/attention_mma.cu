@@ -1,0 +1,340 @@
+// Attention over packed clouds on the tensor cores: 16-bit inputs, width a
+// multiple of 8 up to 128, rows on 16-byte boundaries.
+//
+// Forward: a block owns 256 query rows of one (cloud, head) as two tiles of 128
+// and passes once over the keys in tiles of 128.  S = Q K^T and O += P V are
+// tcgen05 products with fp32 accumulators in tensor memory; P returns to tensor
+// memory as the A operand, over the columns of S that it was made from.  While
+// one tile's softmax runs, the tensor core works for the other tile.
+#include <type_traits>
+
+#include "attention_common.cuh"
+#include "tcgen05.cuh"
+
+namespace tpo {
+namespace {
+
+constexpr int kTile = 128;                        // rows of Q per softmax group, keys per step
+constexpr int kPanel = kTile * kPanelRow;         // 16 KB: 128 rows x 64 elements
+
+// 128 rows of a packed tensor into a swizzled tile by `threads` threads (t = index).
+// Rows at or beyond `valid` and columns at or beyond D become zeros: nothing from
+// another cloud enters a product (0 * NaN would).
+template <typename T, int DP>
+__device__ __forceinline__ void copy_tile(uint32_t dst, const T* src, int64_t stride, int64_t valid, int D, int t) {
+  constexpr int CH = DP / 8;          // 16-byte chunks per row
+  constexpr int STEP = 128 / CH;      // rows per pass of 128 threads
+  const int c = t % CH, r0 = t / CH;
+  const uint32_t at = dst + (c >> 3) * kPanel;
+  const bool col = c * 8 < D;
+  const T* p = src + (int64_t)r0 * stride + c * 8;
+#pragma unroll
+  for (int i = 0; i < CH; ++i) {
+    const int r = r0 + i * STEP;
+    const bool in = col && r < valid;
+    cp_async16(at + r * kPanelRow + (((c & 7) ^ (r & 7)) << 4), in ? (const void*)(p + (int64_t)i * STEP * stride) : (const void*)src, in);
+  }
+}
+
+// ---------------------------------------------------------------- forward
+template <int DP>
+struct FwdSmem {
+  static constexpr int q = kTile * DP * 2;          // one query tile
+  static constexpr int kv = kTile * DP * 2;         // one key or value tile
+  static constexpr int stages = DP == 128 ? 5 : 8;  // tiles in flight
+  static constexpr int bars = 2 * q + stages * kv;
+  static constexpr int total = bars + 256 + 1024;   // + alignment of the base
+};
+constexpr int kFwdThreads = 32 * 13;  // 2 x 4 softmax warps, 4 copy warps, 1 MMA warp
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kFwdThreads, 1) packed_mma_fwd_kernel(const PackedArgs a) {
+  using Sm = FwdSmem<DP>;
+  constexpr int ST = Sm::stages;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_addr(smem_raw);
+  const uint32_t base = (raw + 1023) & ~1023u;
+  const uint32_t sq = base, skv = base + 2 * Sm::q, bars = base + Sm::bars;
+  // barriers: queries full, stages full, stages empty, S full x 2, P full x 2, O done x 2
+  const uint32_t b_q = bars, b_full = bars + 8, b_empty = b_full + 8 * ST, b_s = b_empty + 8 * ST, b_p = b_s + 16,
+                 b_o = b_p + 16, s_tmem = b_o + 16, s_abort = s_tmem + 4;
+  volatile int* abort = reinterpret_cast<volatile int*>(smem_raw + (s_abort - raw));
+  unsigned* err = &g_attention_error;
+
+  const int warp = threadIdx.x / 32, head = blockIdx.y, kvh = head / (a.H / a.Hk);
+  const int64_t slot = a.causal ? (int64_t)gridDim.x - 1 - blockIdx.x : blockIdx.x;
+  const Tile t = find_tile(a.off_q, a.Tq, a.off_k, a.Tk, a.B, 2 * kTile, slot);
+  if (t.rows <= 0) return;
+  const int64_t shift = t.nb - t.na, first = t.row0 - t.a0;
+  // keys that tile w meets, and its steps
+  int64_t nk[2];
+  int steps[2];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const int rows = max(0, min(kTile, t.rows - w * kTile));
+    nk[w] = rows == 0 ? 0 : a.causal ? min64(t.nb, max64(first + w * kTile + rows + shift, 0)) : t.nb;
+    steps[w] = (int)((nk[w] + kTile - 1) / kTile);
+  }
+  const int n = max(steps[0], steps[1]);
+
+  if (warp == 12) {
+    if (threadIdx.x % 32 == 0) {
+      bar_init(b_q, 128);
+      for (int i = 0; i < ST; ++i) {
+        bar_init(b_full + 8 * i, 128);
+        bar_init(b_empty + 8 * i, 1);
+      }
+      for (int w = 0; w < 2; ++w) {
+        bar_init(b_s + 8 * w, 1);
+        bar_init(b_p + 8 * w, 128);
+        bar_init(b_o + 8 * w, 1);
+      }
+      *abort = 0;
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    tmem_alloc(s_tmem, 512);
+    tc_fence_before();
+  }
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(s_tmem));
+  // columns: S0 | S1 | O0 | O1; P over the first half of its S
+  const uint32_t t_s = tmem, t_o = tmem + 256;
+
+  if (warp >= 8 && warp < 12) {
+    // ---- copies: Q, then K0 V0 K1 V1 ... through the ring ----
+    const int tid = threadIdx.x - 256;
+    const T* qp = (const T*)a.q + t.row0 * a.q_st + head * a.q_sh;
+    const T* kp = (const T*)a.k + t.b0 * a.k_st + kvh * a.k_sh;
+    const T* vp = (const T*)a.v + t.b0 * a.v_st + kvh * a.v_sh;
+    if (n > 0) {
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+        copy_tile<T, DP>(sq + w * Sm::q, qp + (int64_t)w * kTile * a.q_st, a.q_st, t.rows - w * kTile, a.D, tid);
+      cp_async_commit();
+      int told = -1;  // tiles below this one are announced; -1: Q is not yet
+      auto announce = [&](int upto) {  // all copies of tiles < upto have landed
+        fence_async_smem();
+        if (told < 0) bar_arrive(b_q), told = 0;
+        for (; told < upto; ++told) bar_arrive(b_full + 8 * (told % ST));
+      };
+      for (int i = 0; i < 2 * n; ++i) {
+        const int s = i % ST;
+        if (i >= ST) {
+          const uint32_t parity = (i / ST - 1) & 1;
+          if (!bar_try(b_empty + 8 * s, parity)) {
+            cp_async_wait<0>();
+            announce(i);
+            bar_wait(b_empty + 8 * s, parity, abort, err);
+          }
+        }
+        const int64_t j = (int64_t)(i >> 1) * kTile;
+        if (i & 1) copy_tile<T, DP>(skv + s * Sm::kv, vp + j * a.v_st, a.v_st, t.nb - j, a.D, tid);
+        else copy_tile<T, DP>(skv + s * Sm::kv, kp + j * a.k_st, a.k_st, t.nb - j, a.D, tid);
+        cp_async_commit();
+        cp_async_wait<1>();
+        announce(i);
+      }
+      cp_async_wait<0>();
+      announce(2 * n);
+    }
+  } else if (warp == 12) {
+    // ---- products, issued by one thread ----
+    if (threadIdx.x % 32 == 0 && n > 0) {
+      constexpr uint32_t id_s = mma_desc<T>(kTile, kTile, false), id_o = mma_desc<T>(kTile, DP, true);
+      auto score = [&](int w, int j) {  // S_w = Q_w K_j^T
+        const uint32_t k = skv + ((2 * j) % ST) * Sm::kv, q = sq + w * Sm::q;
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          const uint32_t at = (ks / 4) * kPanel + (ks % 4) * 32;
+          mma_ss(t_s + w * kTile, smem_desc(q + at, 16), smem_desc(k + at, 16), id_s, ks > 0);
+        }
+      };
+      auto wait_tile = [&](int i) { bar_wait(b_full + 8 * (i % ST), (i / ST) & 1, abort, err); };
+      bar_wait(b_q, 0, abort, err);
+      wait_tile(0);
+      for (int w = 0; w < 2; ++w)
+        if (steps[w] > 0) {
+          score(w, 0);
+          mma_commit(b_s + 8 * w);
+        }
+      // a stage is handed back only where another tile will fill it, so that no
+      // arrival is still on its way when the block ends
+      auto release = [&](int i) {
+        if (i + ST < 2 * n) mma_commit(b_empty + 8 * (i % ST));
+      };
+      release(0);
+      for (int j = 0; j < n; ++j) {
+        const int iv = 2 * j + 1, ik = 2 * j + 2;
+        wait_tile(iv);
+        if (j + 1 < n) wait_tile(ik);
+        const uint32_t v = skv + (iv % ST) * Sm::kv;
+        for (int w = 0; w < 2; ++w) {
+          if (j >= steps[w]) continue;
+          bar_wait(b_p + 8 * w, j & 1, abort, err);
+          tc_fence_after();
+#pragma unroll
+          for (int ks = 0; ks < kTile / 16; ++ks)
+            mma_ts(t_o + w * DP, t_s + w * kTile + ks * 8, smem_desc(v + ks * 16 * kPanelRow, kPanel), id_o,
+                   j > 0 || ks > 0);
+          if (j + 1 < steps[w]) {
+            score(w, j + 1);
+            mma_commit(b_s + 8 * w);
+          } else {
+            mma_commit(b_o + 8 * w);
+          }
+        }
+        release(iv);
+        release(ik);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---- softmax: a thread owns a row ----
+    const int w = warp / 4, row = threadIdx.x % kTile;
+    const uint32_t lane = (uint32_t)(warp % 4) * 32 << 16;
+    const uint32_t ts = t_s + w * kTile + lane, to = t_o + w * DP + lane;
+    const bool live = w * kTile + row < t.rows;
+    const float qscale = a.scale * kLog2e;
+    // this row sees keys below `sees`
+    const int64_t sees = a.causal ? min64(t.nb, first + w * kTile + row + shift + 1) : t.nb;
+    float m = -INFINITY, l = 0.f;
+    for (int j = 0; j < steps[w]; ++j) {
+      bar_wait(b_s + 8 * w, j & 1, abort, err);
+      tc_fence_after();
+      const int64_t left = sees - (int64_t)j * kTile;
+      const int lim = left >= kTile ? kTile : left > 0 ? (int)left : 0;
+      const bool whole = __all_sync(0xffffffffu, lim == kTile);
+      float mx = m;
+#pragma unroll
+      for (int c = 0; c < kTile; c += 32) {
+        uint32_t v[32];
+        tmem_ld32(ts + c, v);
+        tmem_wait_ld();
+        if (whole) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(v[i]));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, c + i < lim ? __uint_as_float(v[i]) : -INFINITY);
+        }
+      }
+      // The base of the exponentials moves only when a maximum outgrows it by
+      // more than 2^8: P stays below 256 (exact scaling by a power of the base is
+      // undone by the division), and O is seldom rescaled.
+      const bool grow = (mx - m) * qscale > 8.f;  // also the first finite maximum: m = -inf
+      if (__any_sync(0xffffffffu, grow)) {
+        const float corr = grow ? ex2((m - mx) * qscale) : 1.f;
+        if (grow) m = mx;
+        l *= corr;
+        if (j > 0) {
+#pragma unroll
+          for (int c = 0; c < DP; c += 32) {
+            uint32_t v[32];
+            tmem_ld32(to + c, v);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
+            tmem_st32(to + c, v);
+          }
+        }
+      }
+      const float mb = m == -INFINITY ? 0.f : m * qscale;
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < kTile; c += 32) {
+        uint32_t v[32], p[16];
+        tmem_ld32(ts + c, v);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float x = ex2(fmaf(__uint_as_float(v[i]), qscale, -mb)), y = ex2(fmaf(__uint_as_float(v[i + 1]), qscale, -mb));
+          if (!whole) {
+            x = c + i < lim ? x : 0.f;
+            y = c + i + 1 < lim ? y : 0.f;
+          }
+          sum += x + y;
+          p[i / 2] = pack2<T>(x, y);
+        }
+        tmem_st16(ts + c / 2, p);
+      }
+      l += sum;
+      tmem_wait_st();
+      tc_fence_before();
+      bar_arrive(b_p + 8 * w);
+    }
+    if (live && a.lse) a.lse[(int64_t)head * a.Tq + t.row0 + w * kTile + row] =
+        l == 0.f ? -INFINITY : (m * qscale + log2f(l)) * kLn2;
+    const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+    T* op = (T*)a.o + ((t.row0 + w * kTile + row) * a.H + head) * a.D;
+    if (steps[w] > 0) {
+      bar_wait(b_o + 8 * w, 0, abort, err);
+      tc_fence_after();
+    }
+#pragma unroll
+    for (int c = 0; c < DP; c += 32) {
+      uint32_t v[32];
+      if (steps[w] > 0) {
+        tmem_ld32(to + c, v);
+        tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = 0;
+      }
+      if (live) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+          if (c + i >= a.D) continue;
+          uint4 o;
+          uint32_t* ov = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            ov[e] = pack2<T>(__uint_as_float(v[i + 2 * e]) * inv, __uint_as_float(v[i + 2 * e + 1]) * inv);
+          *reinterpret_cast<uint4*>(op + c + i) = o;
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 12) {
+    tc_fence_after();
+    tmem_free(tmem, 512);
+  }
+}
+
+template <typename K>
+int set_smem(K kern, int bytes) {
+  return cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+}
+
+template <typename T, int DP>
+int fwd(const PackedArgs& a, cudaStream_t st) {
+  auto kern = packed_mma_fwd_kernel<T, DP>;
+  int s = set_smem(kern, FwdSmem<DP>::total);
+  if (s) return s;
+  kern<<<dim3((unsigned)packed_slots(a.Tq, a.B, 2 * kTile), a.H), kFwdThreads, FwdSmem<DP>::total, st>>>(a);
+  return check_launch();
+}
+
+bool rows16(const void* p, int64_t s1, int64_t s2) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s1 % 8 == 0 && s2 % 8 == 0;
+}
+
+}  // namespace
+
+bool packed_mma_takes(int dtype, const PackedArgs& a, bool backward) {
+  return (dtype == TPO_F16 || dtype == TPO_BF16) && a.D % 8 == 0 && a.D <= 128 && rows16(a.q, a.q_st, a.q_sh) &&
+         rows16(a.k, a.k_st, a.k_sh) && rows16(a.v, a.v_st, a.v_sh) && (!backward || rows16(a.go, a.go_st, a.go_sh));
+}
+
+int packed_mma_forward(int dtype, const PackedArgs& a, cudaStream_t st) {
+  if (dtype == TPO_F16) return a.D <= 64 ? fwd<__half, 64>(a, st) : fwd<__half, 128>(a, st);
+  return a.D <= 64 ? fwd<__nv_bfloat16, 64>(a, st) : fwd<__nv_bfloat16, 128>(a, st);
+}
+
+int attention_mma_error_flags(unsigned* out, bool clear) { return read_attention_error(out, clear); }
+
+}  // namespace tpo

@@ -49,12 +49,13 @@ const char* tpo_status_string(int status) {
 
 int tpo_device_error_flags(unsigned* flags, int clear) {
   if (!flags) return fail(TPO_ERR_INVALID_ARGUMENT, "device_error_flags: null output");
-  unsigned a = 0, b = 0, c = 0, d = 0;
+  unsigned a = 0, b = 0, c = 0, d = 0, e = 0;
   int s = device_error_flags(&a, clear != 0);
   if (!s) s = fps_device_error_flags(&b, clear != 0);
   if (!s) s = knn_device_error_flags(&c, clear != 0);
   if (!s) s = attention_simt_error_flags(&d, clear != 0);
-  *flags = a | b | c | d;
+  if (!s) s = attention_mma_error_flags(&e, clear != 0);
+  *flags = a | b | c | d | e;
   return s;
 }
 

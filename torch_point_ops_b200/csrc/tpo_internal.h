@@ -100,6 +100,7 @@ int cached_attention(int dtype, const void* q, const int64_t* q_stride, const vo
                      const int64_t* lengths, int64_t N, int64_t P, int64_t H, int64_t Hk, int64_t D,
                      float scale, void* o, void* ws, cudaStream_t st);
 int attention_simt_error_flags(unsigned* out, bool clear);
+int attention_mma_error_flags(unsigned* out, bool clear);
 
 // Launches `kern` with programmatic stream serialisation allowed (see pdl_wait).
 template <typename... KArgs, typename... Args>

@@ -23,7 +23,7 @@ struct PackedArgs {
   const int64_t *off_q, *off_k;
   void *o, *dq, *dk, *dv;
   float *lse, *delta;
-  const unsigned* go_max;  // largest |go| as bits of a float (fp16 backward), or null
+  float* go_max;  // (H, Tq): largest |go| of each row (fp16 on the tensor cores), or null
   int64_t Tq, Tk;
   int B, H, Hk, D, causal;
   float scale;
@@ -96,6 +96,7 @@ int packed_simt_backward(int dtype, const PackedArgs& a, cudaStream_t st);
 // Whether the tensor-core kernels take the problem, and those kernels.
 bool packed_mma_takes(int dtype, const PackedArgs& a, bool backward);
 int packed_mma_forward(int dtype, const PackedArgs& a, cudaStream_t st);
+int packed_mma_backward(int dtype, const PackedArgs& a, cudaStream_t st);
 int packed_delta(int dtype, const PackedArgs& a, cudaStream_t st);
 
 }  // namespace tpo

@@ -331,21 +331,41 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
   }
 }
 
-// delta = dO . O per (head, token): a warp per row.
-template <typename T>
-__global__ void __launch_bounds__(256) packed_delta_kernel(const PackedArgs a) {
+// delta = dO . O per (head, token), and the row's largest |dO| where asked for; lpr
+// lanes per row, vectors of VEC.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) packed_delta_kernel(const PackedArgs a, int lpr) {
   const int64_t rows = a.Tq * a.H;
-  const int lane = threadIdx.x & 31;
-  for (int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; r < rows; r += (int64_t)gridDim.x * 8) {
-    const int64_t tok = r / a.H;
-    const int head = (int)(r - tok * a.H);
-    const T* o = (const T*)a.o + r * a.D;
-    const T* g = (const T*)a.go + tok * a.go_st + head * a.go_sh;
-    float s = 0.f;
-    for (int c = lane; c < a.D; c += 32) s += to_acc(o[c]) * to_acc(g[c]);
+  const int rpb = 256 / lpr, l = threadIdx.x % lpr;
+  for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < rows; r0 += (int64_t)gridDim.x * rpb) {
+    const int64_t r = r0 + threadIdx.x / lpr;
+    float s = 0.f, big = 0.f;
+    int64_t tok = 0;
+    int head = 0;
+    if (r < rows) {
+      tok = r / a.H;
+      head = (int)(r - tok * a.H);
+      const T* o = (const T*)a.o + r * a.D;
+      const T* g = (const T*)a.go + tok * a.go_st + head * a.go_sh;
+      for (int c = l * VEC; c < a.D; c += lpr * VEC) {
+        float x[VEC], y[VEC];
+        load_vec<VEC>(o + c, x);
+        load_vec<VEC>(g + c, y);
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    if (lane == 0) a.delta[(int64_t)head * a.Tq + tok] = s;
+        for (int i = 0; i < VEC; ++i) {
+          s += x[i] * y[i];
+          big = fmaxf(big, fabsf(y[i]));
+        }
+      }
+    }
+    for (int x = lpr / 2; x > 0; x >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, x);
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+    }
+    if (r < rows && l == 0) {
+      a.delta[(int64_t)head * a.Tq + tok] = s;
+      if (a.go_max) a.go_max[(int64_t)head * a.Tq + tok] = big;
+    }
   }
 }
 
@@ -418,10 +438,20 @@ int bwd_typed(const PackedArgs& a, cudaStream_t st) {
   return vec_ok<T>(a, true) ? bwd_width<T, 16 / sizeof(T)>(a, st) : bwd_width<T, 1>(a, st);
 }
 
+template <typename T, int VEC>
+int delta_launch(const PackedArgs& a, cudaStream_t st) {
+  int lpr = 32;
+  while (lpr > 1 && (lpr / 2) * VEC >= a.D) lpr /= 2;
+  const int rpb = 256 / lpr;
+  packed_delta_kernel<T, VEC><<<(unsigned)min64((a.Tq * a.H + rpb - 1) / rpb, 148 * 16), 256, 0, st>>>(a, lpr);
+  return check_launch();
+}
 template <typename T>
 int delta_typed(const PackedArgs& a, cudaStream_t st) {
-  packed_delta_kernel<T><<<(unsigned)min64((a.Tq * a.H + 7) / 8, 148 * 32), 256, 0, st>>>(a);
-  return check_launch();
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = a.D % V == 0 && (reinterpret_cast<uintptr_t>(a.go) & 15) == 0 &&
+                   (reinterpret_cast<uintptr_t>(a.o) & 15) == 0 && a.go_st % V == 0 && a.go_sh % V == 0;
+  return vec ? delta_launch<T, V>(a, st) : delta_launch<T, 1>(a, st);
 }
 
 }  // namespace

@@ -13,6 +13,7 @@
 //
 // Slots at or beyond lengths[n] are never read: they may hold anything.
 #include "attention_common.cuh"
+#include "tcgen05.cuh"  // pack2
 
 namespace tpo {
 namespace {
@@ -195,6 +196,209 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const CachedArgs 
   }
 }
 
+// ---------------------------------------------------------------------------
+// 16-bit types, D a multiple of 8 up to 128, rows on 16-byte boundaries: the heads
+// of a group (16 to a block) are the M rows of m16n8k16 products, so the work per
+// cached byte stays small for any group.  A warp takes 16 keys at a time.
+//
+// Both products take their cache operand straight from 16-byte global loads; what
+// the fragments want is met by permuting the summed or the free index:
+//   S = Q K^T: lane (g = lane/4, c = lane%4) loads chunks 4i + c (8 elements each) of
+//     key g; a chunk's register pairs serve as two k-steps, with Q's chunks loaded in
+//     the same order.
+//   O = P V: the score fragment is the A fragment (keys 2c, 2c+1, 2c+8, 2c+9 of lane
+//     c); lane (g, c) loads chunk 8h + g of those four keys, and product t of half h takes
+//     element t of every chunk as its column, so a lane ends with whole chunks 8h + 2c
+//     and 8h + 2c + 1 of rows g and g + 8.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint4 load16(const void* p, bool in) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (in)
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                 uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                                        uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <typename T, int DP, bool TALL>  // TALL: the block has more than 8 heads
+__global__ void __launch_bounds__(kThreads) cached_mma_kernel(const CachedArgs a) {
+  constexpr int KC = DP / 32, VC = DP / 64;
+  __shared__ float jm[kWarps][16], jl[kWarps][16];
+  __shared__ float jo[kWarps][TALL ? 16 : 8][DP + 4];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, c = lane % 4;
+  const int group = a.H / a.Hk, gblocks = (group + 15) / 16;
+  const int n = blockIdx.y, kvh = blockIdx.z / gblocks, g0 = (blockIdx.z % gblocks) * 16;
+  const int gn = min(16, group - g0);
+  const int64_t len = length_of(a, n);
+  const int64_t j_begin = (int64_t)blockIdx.x * a.chunk, j_end = min64(len, j_begin + a.chunk);
+  if (blockIdx.x > 0 && j_begin >= len) return;  // the join skips this chunk too
+  const T* kp = (const T*)a.k + n * a.k_sn + kvh * a.k_sh;
+  const T* vp = (const T*)a.v + n * a.v_sn + kvh * a.v_sh;
+  uint4 q[TALL ? 2 : 1][KC];
+#pragma unroll
+  for (int r = 0; r < (TALL ? 2 : 1); ++r)
+#pragma unroll
+    for (int i = 0; i < KC; ++i) {
+      const int ch = 4 * i + c, row = g + 8 * r;
+      q[r][i] = load16((const T*)a.q + n * a.q_sn + (kvh * group + g0 + row) * a.q_sh + ch * 8, row < gn && ch * 8 < a.D);
+    }
+  float acc[VC][8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+  for (int h = 0; h < VC; ++h)
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[h][t][e] = 0.f;
+
+  for (int64_t j0 = j_begin + warp * 16; j0 < j_end; j0 += kWarps * 16) {
+    const int left = (int)min64(16, j_end - j0);
+    uint4 kk[2][KC], vv[4][VC];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        const int key = 8 * b + g, ch = 4 * i + c;
+        kk[b][i] = load16(kp + (j0 + key) * a.k_sp + ch * 8, key < left && ch * 8 < a.D);
+      }
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int h = 0; h < VC; ++h) {
+        const int key = 2 * c + (b & 1) + 8 * (b >> 1), ch = 8 * h + g;
+        vv[b][h] = load16(vp + (j0 + key) * a.v_sp + ch * 8, key < left && ch * 8 < a.D);
+      }
+    float s[2][4];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[b][e] = 0.f;
+#pragma unroll
+      for (int i = 0; i < KC; ++i) {
+        const uint4 x = q[0][i], y = TALL ? q[TALL ? 1 : 0][i] : make_uint4(0, 0, 0, 0);
+        mma16816<T>(s[b], x.x, y.x, x.y, y.y, kk[b][i].x, kk[b][i].y);
+        mma16816<T>(s[b], x.z, y.z, x.w, y.w, kk[b][i].z, kk[b][i].w);
+      }
+    }
+    // rows g (e = 0, 1) and g + 8 (e = 2, 3); keys 8 b + 2 c + (e & 1)
+    float p[2][4];
+    bool moved = false;
+    float corr[2] = {1.f, 1.f};
+#pragma unroll
+    for (int r = 0; r < (TALL ? 2 : 1); ++r) {
+      float mx = m[r];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float& x = s[b][2 * r + e];
+          x = 8 * b + 2 * c + e < left ? x * a.qscale : -INFINITY;
+          mx = fmaxf(mx, x);
+        }
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float base = mx == -INFINITY ? 0.f : mx;
+      if (mx != m[r]) {
+        corr[r] = exp2f(m[r] - base);
+        moved = true;
+      }
+      m[r] = mx;
+      float sum = 0.f;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) sum += p[b][2 * r + e] = exp2f(s[b][2 * r + e] - base);
+      l[r] = l[r] * corr[r] + sum;  // this lane's keys
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int h = 0; h < VC; ++h)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          acc[h][t][0] *= corr[0], acc[h][t][1] *= corr[0];
+          if (TALL) acc[h][t][2] *= corr[1], acc[h][t][3] *= corr[1];
+        }
+    }
+    // P is rounded to the cache's type here; its sum is not
+    const uint32_t a0 = pack2<T>(p[0][0], p[0][1]), a2 = pack2<T>(p[1][0], p[1][1]);
+    const uint32_t a1 = TALL ? pack2<T>(p[0][2], p[0][3]) : 0u, a3 = TALL ? pack2<T>(p[1][2], p[1][3]) : 0u;
+#pragma unroll
+    for (int h = 0; h < VC; ++h) {
+      const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vv[0][h]);
+      const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vv[1][h]);
+      const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&vv[2][h]);
+      const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&vv[3][h]);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        mma16816<T>(acc[h][2 * x], a0, a1, a2, a3, __byte_perm(v0[x], v1[x], 0x5410), __byte_perm(v2[x], v3[x], 0x5410));
+        mma16816<T>(acc[h][2 * x + 1], a0, a1, a2, a3, __byte_perm(v0[x], v1[x], 0x7632), __byte_perm(v2[x], v3[x], 0x7632));
+      }
+    }
+  }
+  // the warps' rows, joined in order
+#pragma unroll
+  for (int r = 0; r < (TALL ? 2 : 1); ++r) {
+    float x = l[r];
+    x += __shfl_xor_sync(0xffffffffu, x, 1);
+    x += __shfl_xor_sync(0xffffffffu, x, 2);
+    if (c == 0) {
+      jm[warp][g + 8 * r] = m[r];
+      jl[warp][g + 8 * r] = x;
+    }
+#pragma unroll
+    for (int h = 0; h < VC; ++h)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float* o = &jo[warp][g + 8 * r][(8 * h + 2 * c + e) * 8];
+#pragma unroll
+        for (int t = 0; t < 8; t += 4)
+          *reinterpret_cast<float4*>(o + t) = make_float4(acc[h][t][2 * r + e], acc[h][t + 1][2 * r + e],
+                                                          acc[h][t + 2][2 * r + e], acc[h][t + 3][2 * r + e]);
+      }
+  }
+  __syncthreads();
+  const int64_t row0 = (int64_t)n * a.H + kvh * group + g0;
+  for (int i = threadIdx.x; i < gn * (DP / 4); i += kThreads) {
+    const int row = i / (DP / 4), col = (i % (DP / 4)) * 4;
+    if (col >= a.D) continue;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, jm[w][row]);
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f}, ls = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = exp2f(jm[w][row] - base);
+      const float4 o = *reinterpret_cast<const float4*>(&jo[w][row][col]);
+      sum[0] += f * o.x, sum[1] += f * o.y, sum[2] += f * o.z, sum[3] += f * o.w;
+      ls += f * jl[w][row];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) put<T>(a, row0 + row, blockIdx.x, col + e, sum[e], ls);
+    if (a.chunks > 1 && col == 0) {
+      float* st = part_stats(a) + ((row0 + row) * a.chunks + blockIdx.x) * 2;
+      st[0] = mx;
+      st[1] = ls;
+    }
+  }
+}
+
 // Joins the chunks of a head's row: o = sum_c 2^(m_c - m) sum_c / sum_c 2^(m_c - m) l_c.
 // A block per row; eight strands of chunks, joined in order.
 template <typename T>
@@ -284,10 +488,26 @@ bool aligned16(const CachedArgs& a) {
          (a.q_sn | a.q_sh | a.k_sn | a.k_sp | a.k_sh | a.v_sn | a.v_sp | a.v_sh) % V == 0;
 }
 
+template <typename T, int DP>
+int mma_launch(const CachedArgs& a, cudaStream_t st) {
+  const int group = a.H / a.Hk;
+  const dim3 grid(a.chunks, a.N, a.Hk * ((group + 15) / 16));
+  if (group > 8) cached_mma_kernel<T, DP, true><<<grid, kThreads, 0, st>>>(a);
+  else cached_mma_kernel<T, DP, false><<<grid, kThreads, 0, st>>>(a);
+  return check_launch();
+}
+
 template <typename T>
 int cached_typed(const CachedArgs& a, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
   int s;
+  if constexpr (sizeof(T) == 2) {
+    if (a.D <= 128 && aligned16<T>(a)) {
+      s = a.D <= 64 ? mma_launch<T, 64>(a, st) : mma_launch<T, 128>(a, st);
+      if (s || a.chunks == 1) return s;
+      return launch_pdl(cached_join_kernel<T>, dim3((unsigned)(a.N * a.H)), dim3(256), 0, st, a);
+    }
+  }
   if (aligned16<T>(a)) {
     if (a.D <= 16 * V) s = simt_group<T, V, 16, 1>(a, st);
     else if (a.D <= 32 * V) s = simt_group<T, V, 32, 1>(a, st);

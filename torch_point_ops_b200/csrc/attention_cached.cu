@@ -25,7 +25,7 @@ struct CachedArgs {
   int64_t q_sn, q_sh, k_sn, k_sp, k_sh, v_sn, v_sp, v_sh;
   const int64_t* lengths;
   void* o;
-  float* part;  // (N*H, chunks, D) sums, then (N*H, chunks, 2) maxima (base 2) and weights
+  float* part;  // (N*H, chunks, pitch) sums, then (N*H, chunks, 2) maxima (base 2) and weights
   int64_t P, chunk;
   int N, H, Hk, D, chunks;
   float qscale;  // scale * log2(e)
@@ -34,8 +34,9 @@ struct CachedArgs {
 __device__ __forceinline__ int64_t length_of(const CachedArgs& a, int n) {
   return min64(max64(a.lengths[n], 0), a.P);
 }
+__host__ __device__ __forceinline__ int part_pitch(int D) { return (D + 3) & ~3; }  // rows on 16 bytes
 __device__ __forceinline__ float* part_stats(const CachedArgs& a) {
-  return a.part + (int64_t)a.N * a.H * a.chunks * a.D;
+  return a.part + (int64_t)a.N * a.H * a.chunks * part_pitch(a.D);
 }
 
 // Writes one head's row: the result itself when the key axis is one chunk, else
@@ -45,7 +46,7 @@ __device__ __forceinline__ void put(const CachedArgs& a, int64_t row, int chunk,
   if (a.chunks == 1)
     ((T*)a.o)[row * a.D + c] = from_acc<T>(l > 0.f ? sum / l : l == 0.f ? 0.f : l);
   else
-    a.part[(row * a.chunks + chunk) * a.D + c] = sum;
+    a.part[(row * a.chunks + chunk) * part_pitch(a.D) + c] = sum;
 }
 
 // ---------------------------------------------------------------------------
@@ -57,6 +58,7 @@ __device__ __forceinline__ void put(const CachedArgs& a, int64_t row, int chunk,
 // ---------------------------------------------------------------------------
 template <typename T, int VEC, int LPK, int NVL, int GB>
 __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const CachedArgs a) {
+  constexpr int UNR = GB <= 2 ? 8 : 4;
   constexpr int KPI = 32 / LPK, W = LPK * NVL * VEC;
   __shared__ float sc[kWarps][GB][32];
   __shared__ float jm[kWarps][GB], jl[kWarps][GB];
@@ -64,11 +66,11 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const CachedArgs 
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int kl = lane % LPK, kr = lane / LPK;
   const int group = a.H / a.Hk, gblocks = (group + GB - 1) / GB;
-  const int n = blockIdx.y, kvh = blockIdx.z / gblocks, g0 = (blockIdx.z % gblocks) * GB;
+  const int n = blockIdx.z, kvh = blockIdx.x / gblocks, g0 = (blockIdx.x % gblocks) * GB, chunk = blockIdx.y;
   const int gn = min(GB, group - g0);
   const int64_t len = length_of(a, n);
-  const int64_t j_begin = (int64_t)blockIdx.x * a.chunk, j_end = min64(len, j_begin + a.chunk);
-  if (blockIdx.x > 0 && j_begin >= len) return;  // the join skips this chunk too
+  const int64_t j_begin = (int64_t)chunk * a.chunk, j_end = min64(len, j_begin + a.chunk);
+  if (chunk > 0 && j_begin >= len) return;  // the join skips this chunk too
   const int64_t row0 = (int64_t)n * a.H + kvh * group + g0;
   float q[GB][NVL][VEC], acc[GB][NVL][VEC], m[GB], l[GB];
 #pragma unroll
@@ -87,25 +89,23 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const CachedArgs 
   const T* kp = (const T*)a.k + n * a.k_sn + kvh * a.k_sh;
   const T* vp = (const T*)a.v + n * a.v_sn + kvh * a.v_sh;
   for (int64_t j0 = j_begin + warp * 32; j0 < j_end; j0 += kWarps * 32) {
-#pragma unroll 4
+#pragma unroll(UNR)
     for (int i = 0; i < 32; i += KPI) {
-      const int64_t j = j0 + i + kr;
+      // unconditional, so that the loads of several steps are in flight together; a key
+      // beyond the end repeats the last one and is masked below
+      const T* row = kp + min64(j0 + i + kr, j_end - 1) * a.k_sp;
       float s[GB];
 #pragma unroll
       for (int g = 0; g < GB; ++g) s[g] = 0.f;
-      if (j < j_end) {
 #pragma unroll
-        for (int x = 0; x < NVL; ++x) {
-          const int c = (x * LPK + kl) * VEC;
-          float kv[VEC];
+      for (int x = 0; x < NVL; ++x) {
+        const int c = (x * LPK + kl) * VEC;
+        float kv[VEC];
+        load_vec<VEC>(row + (c < a.D ? c : 0), kv);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) kv[e] = 0.f;
-          if (c < a.D) load_vec<VEC>(kp + j * a.k_sp + c, kv);
+        for (int g = 0; g < GB; ++g)
 #pragma unroll
-          for (int g = 0; g < GB; ++g)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) s[g] = fmaf(q[g][x][e], kv[e], s[g]);
-        }
+          for (int e = 0; e < VEC; ++e) s[g] = fmaf(q[g][x][e], c < a.D ? kv[e] : 0.f, s[g]);
       }
 #pragma unroll
       for (int g = 0; g < GB; ++g) {
@@ -132,23 +132,21 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const CachedArgs 
         for (int e = 0; e < VEC; ++e) acc[g][x][e] *= corr;
     }
     __syncwarp();
-#pragma unroll 4
+#pragma unroll(UNR)
     for (int i = 0; i < 32; i += KPI) {
-      const int64_t j = j0 + i + kr;
-      if (j < j_end) {
+      // as above; the repeated last key has probability 0 in the repeats (a value that is
+      // not finite there is in the result anyway), columns beyond D are never written
+      const T* row = vp + min64(j0 + i + kr, j_end - 1) * a.v_sp;
 #pragma unroll
-        for (int x = 0; x < NVL; ++x) {
-          const int c = (x * LPK + kl) * VEC;
-          float vv[VEC];
+      for (int x = 0; x < NVL; ++x) {
+        const int c = (x * LPK + kl) * VEC;
+        float vv[VEC];
+        load_vec<VEC>(row + (c < a.D ? c : 0), vv);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) vv[e] = 0.f;
-          if (c < a.D) load_vec<VEC>(vp + j * a.v_sp + c, vv);
+        for (int g = 0; g < GB; ++g) {
+          const float p = sc[warp][g][i + kr];
 #pragma unroll
-          for (int g = 0; g < GB; ++g) {
-            const float p = sc[warp][g][i + kr];
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[g][x][e] = fmaf(p, vv[e], acc[g][x][e]);
-          }
+          for (int e = 0; e < VEC; ++e) acc[g][x][e] = fmaf(p, vv[e], acc[g][x][e]);
         }
       }
     }
@@ -187,9 +185,9 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const CachedArgs 
       sum += f * jo[w][g][c];
       ls += f * jl[w][g];
     }
-    put<T>(a, row0 + g, blockIdx.x, c, sum, ls);
+    put<T>(a, row0 + g, chunk, c, sum, ls);
     if (a.chunks > 1 && c == 0) {
-      float* st = part_stats(a) + ((row0 + g) * a.chunks + blockIdx.x) * 2;
+      float* st = part_stats(a) + ((row0 + g) * a.chunks + chunk) * 2;
       st[0] = mx;
       st[1] = ls;
     }
@@ -201,8 +199,12 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const CachedArgs 
 // of a group (16 to a block) are the M rows of m16n8k16 products, so the work per
 // cached byte stays small for any group.  A warp takes 16 keys at a time.
 //
-// Both products take their cache operand straight from 16-byte global loads; what
-// the fragments want is met by permuting the summed or the free index:
+// A warp owns a queue of kStages tiles in shared memory: each lane fetches one row of
+// a tile (16 keys, 16 values) with one bulk copy, so the copies cost a handful of
+// instructions per 8 KB and are not bound by the load unit's outstanding misses.  The
+// row pitches (256 + 64 and 256 + 16 bytes) keep both products' 128-bit reads free of
+// bank conflicts.  What the fragments want is met by permuting the summed or the
+// free index:
 //   S = Q K^T: lane (g = lane/4, c = lane%4) loads chunks 4i + c (8 elements each) of
 //     key g; a chunk's register pairs serve as two k-steps, with Q's chunks loaded in
 //     the same order.
@@ -211,14 +213,6 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const CachedArgs 
 //     element t of every chunk as its column, so a lane ends with whole chunks 8h + 2c
 //     and 8h + 2c + 1 of rows g and g + 8.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ uint4 load16(const void* p, bool in) {
-  uint4 v = make_uint4(0, 0, 0, 0);
-  if (in)
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-  return v;
-}
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1);
@@ -237,27 +231,72 @@ __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], uint32_t 
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+template <int DP>
+struct MmaShape {
+  static constexpr int KC = DP / 32, VC = DP / 64;
+  static constexpr int kp = DP * 2 + 64, vp = DP * 2 + 16;  // row pitches, bytes
+  static constexpr int tile = 16 * (kp + vp);
+  static constexpr int stages = DP == 128 ? 2 : 3;  // three blocks per SM: measured against two blocks with a longer queue
+  static constexpr int smem = kWarps * stages * tile;  // also holds the join: 16 rows of DP + 4 floats per warp
+  static_assert(stages * tile >= 16 * (DP + 4) * 4, "join buffer");
+};
+
 template <typename T, int DP, bool TALL>  // TALL: the block has more than 8 heads
-__global__ void __launch_bounds__(kThreads) cached_mma_kernel(const CachedArgs a) {
-  constexpr int KC = DP / 32, VC = DP / 64;
+__global__ void __launch_bounds__(kThreads, 3) cached_mma_kernel(const CachedArgs a) {
+  using Sh = MmaShape<DP>;
+  constexpr int KC = Sh::KC, VC = Sh::VC, ST = Sh::stages;
   __shared__ float jm[kWarps][16], jl[kWarps][16];
-  __shared__ float jo[kWarps][TALL ? 16 : 8][DP + 4];
+  __shared__ unsigned long long full[kWarps][ST];
+  extern __shared__ uint4 ring[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, c = lane % 4;
   const int group = a.H / a.Hk, gblocks = (group + 15) / 16;
-  const int n = blockIdx.y, kvh = blockIdx.z / gblocks, g0 = (blockIdx.z % gblocks) * 16;
+  const int n = blockIdx.z, kvh = blockIdx.x / gblocks, g0 = (blockIdx.x % gblocks) * 16, chunk = blockIdx.y;
   const int gn = min(16, group - g0);
   const int64_t len = length_of(a, n);
-  const int64_t j_begin = (int64_t)blockIdx.x * a.chunk, j_end = min64(len, j_begin + a.chunk);
-  if (blockIdx.x > 0 && j_begin >= len) return;  // the join skips this chunk too
+  const int64_t j_begin = (int64_t)chunk * a.chunk, j_end = min64(len, j_begin + a.chunk);
+  if (chunk > 0 && j_begin >= len) return;  // the join skips this chunk too
+  pdl_trigger();
   const T* kp = (const T*)a.k + n * a.k_sn + kvh * a.k_sh;
   const T* vp = (const T*)a.v + n * a.v_sn + kvh * a.v_sh;
+  uint8_t* mine = reinterpret_cast<uint8_t*>(ring) + warp * ST * Sh::tile;  // this warp's queue
+  const int64_t j_first = j_begin + warp * 16;
+  if (lane < ST) mbar_init(&full[warp][lane], 1);
+  if (a.D < DP) {  // no copy writes the columns beyond D: zeros, once
+    for (int i = lane; i < ST * Sh::tile / 16; i += 32) reinterpret_cast<uint4*>(mine)[i] = make_uint4(0, 0, 0, 0);
+    fence_async_smem();
+  }
+  __syncwarp();
+  // Lane 0-15: key of the tile, 16-31: value.  Beyond the end: keys are masked
+  // whatever they hold, values become zeros (0 * NaN).
+  const int r = lane & 15;
+  const T* src = lane < 16 ? kp + r * a.k_sp : vp + r * a.v_sp;
+  const int64_t src_step = lane < 16 ? a.k_sp : a.v_sp;
+  const int dst_row = lane < 16 ? r * Sh::kp : 16 * Sh::kp + r * Sh::vp;
+  const unsigned row_bytes = a.D * 2;
+  auto fetch = [&](int64_t j0, int slot) {
+    const int left = (int)min64(16, j_end - j0);
+    uint8_t* dst = mine + slot * Sh::tile + dst_row;
+    if (lane == 0) mbar_expect_tx(&full[warp][slot], 2 * left * row_bytes);
+    __syncwarp();
+    if (r < left) {
+      bulk_g2s(dst, src + j0 * src_step, row_bytes, &full[warp][slot]);
+    } else if (lane >= 16) {  // the warp's last tile: nothing is copied here afterwards
+#pragma unroll
+      for (int i = 0; i < DP * 2; i += 16) *reinterpret_cast<uint4*>(dst + i) = make_uint4(0, 0, 0, 0);
+    }
+  };
+#pragma unroll
+  for (int s = 0; s < ST - 1; ++s)
+    if (j_first + s * kWarps * 16 < j_end) fetch(j_first + s * kWarps * 16, s);
   uint4 q[TALL ? 2 : 1][KC];
 #pragma unroll
   for (int r = 0; r < (TALL ? 2 : 1); ++r)
 #pragma unroll
     for (int i = 0; i < KC; ++i) {
       const int ch = 4 * i + c, row = g + 8 * r;
-      q[r][i] = load16((const T*)a.q + n * a.q_sn + (kvh * group + g0 + row) * a.q_sh + ch * 8, row < gn && ch * 8 < a.D);
+      q[r][i] = make_uint4(0, 0, 0, 0);
+      if (row < gn && ch * 8 < a.D)
+        q[r][i] = *reinterpret_cast<const uint4*>((const T*)a.q + n * a.q_sn + (kvh * group + g0 + row) * a.q_sh + ch * 8);
     }
   float acc[VC][8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
@@ -267,34 +306,33 @@ __global__ void __launch_bounds__(kThreads) cached_mma_kernel(const CachedArgs a
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[h][t][e] = 0.f;
 
-  for (int64_t j0 = j_begin + warp * 16; j0 < j_end; j0 += kWarps * 16) {
+  int slot = 0;
+  unsigned parity = 0;
+  for (int64_t j0 = j_first; j0 < j_end; j0 += kWarps * 16) {
     const int left = (int)min64(16, j_end - j0);
-    uint4 kk[2][KC], vv[4][VC];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int i = 0; i < KC; ++i) {
-        const int key = 8 * b + g, ch = 4 * i + c;
-        kk[b][i] = load16(kp + (j0 + key) * a.k_sp + ch * 8, key < left && ch * 8 < a.D);
-      }
-#pragma unroll
-    for (int b = 0; b < 4; ++b)
-#pragma unroll
-      for (int h = 0; h < VC; ++h) {
-        const int key = 2 * c + (b & 1) + 8 * (b >> 1), ch = 8 * h + g;
-        vv[b][h] = load16(vp + (j0 + key) * a.v_sp + ch * 8, key < left && ch * 8 < a.D);
-      }
+    const int64_t ahead = j0 + (ST - 1) * kWarps * 16;
+    __syncwarp();  // every lane has read the slot that is filled next
+    if (ahead < j_end) fetch(ahead, slot == 0 ? ST - 1 : slot - 1);
+    mbar_wait(&full[warp][slot], parity, &g_attention_error);
+    __syncwarp();
+    const uint8_t* keys = mine + slot * Sh::tile + g * Sh::kp + c * 16;
+    const uint8_t* vals = mine + slot * Sh::tile + 16 * Sh::kp + 2 * c * Sh::vp + g * 16;
+    if (++slot == ST) slot = 0, parity ^= 1;
     float s[2][4];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[b][e] = 0.f;
+      float s2[4] = {0.f, 0.f, 0.f, 0.f};  // two chains of products: each waits for its predecessor
 #pragma unroll
       for (int i = 0; i < KC; ++i) {
         const uint4 x = q[0][i], y = TALL ? q[TALL ? 1 : 0][i] : make_uint4(0, 0, 0, 0);
-        mma16816<T>(s[b], x.x, y.x, x.y, y.y, kk[b][i].x, kk[b][i].y);
-        mma16816<T>(s[b], x.z, y.z, x.w, y.w, kk[b][i].z, kk[b][i].w);
+        const uint4 kk = *reinterpret_cast<const uint4*>(keys + b * 8 * Sh::kp + i * 64);
+        mma16816<T>(s[b], x.x, y.x, x.y, y.y, kk.x, kk.y);
+        mma16816<T>(s2, x.z, y.z, x.w, y.w, kk.z, kk.w);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[b][e] += s2[e];
     }
     // rows g (e = 0, 1) and g + 8 (e = 2, 3); keys 8 b + 2 c + (e & 1)
     float p[2][4];
@@ -340,10 +378,12 @@ __global__ void __launch_bounds__(kThreads) cached_mma_kernel(const CachedArgs a
     const uint32_t a1 = TALL ? pack2<T>(p[0][2], p[0][3]) : 0u, a3 = TALL ? pack2<T>(p[1][2], p[1][3]) : 0u;
 #pragma unroll
     for (int h = 0; h < VC; ++h) {
-      const uint32_t* v0 = reinterpret_cast<const uint32_t*>(&vv[0][h]);
-      const uint32_t* v1 = reinterpret_cast<const uint32_t*>(&vv[1][h]);
-      const uint32_t* v2 = reinterpret_cast<const uint32_t*>(&vv[2][h]);
-      const uint32_t* v3 = reinterpret_cast<const uint32_t*>(&vv[3][h]);
+      uint4 vv[4];
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        vv[b] = *reinterpret_cast<const uint4*>(vals + ((b & 1) + 8 * (b >> 1)) * Sh::vp + h * 128);
+      const uint32_t *v0 = reinterpret_cast<const uint32_t*>(&vv[0]), *v1 = reinterpret_cast<const uint32_t*>(&vv[1]);
+      const uint32_t *v2 = reinterpret_cast<const uint32_t*>(&vv[2]), *v3 = reinterpret_cast<const uint32_t*>(&vv[3]);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         mma16816<T>(acc[h][2 * x], a0, a1, a2, a3, __byte_perm(v0[x], v1[x], 0x5410), __byte_perm(v2[x], v3[x], 0x5410));
@@ -351,7 +391,9 @@ __global__ void __launch_bounds__(kThreads) cached_mma_kernel(const CachedArgs a
       }
     }
   }
-  // the warps' rows, joined in order
+  // the warps' rows, joined in order (every copy has been waited for)
+  __syncthreads();
+  float* jo = reinterpret_cast<float*>(ring);  // [warp][row][DP + 4]
 #pragma unroll
   for (int r = 0; r < (TALL ? 2 : 1); ++r) {
     float x = l[r];
@@ -365,7 +407,7 @@ __global__ void __launch_bounds__(kThreads) cached_mma_kernel(const CachedArgs a
     for (int h = 0; h < VC; ++h)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float* o = &jo[warp][g + 8 * r][(8 * h + 2 * c + e) * 8];
+        float* o = jo + (warp * 16 + g + 8 * r) * (DP + 4) + (8 * h + 2 * c + e) * 8;
 #pragma unroll
         for (int t = 0; t < 8; t += 4)
           *reinterpret_cast<float4*>(o + t) = make_float4(acc[h][t][2 * r + e], acc[h][t + 1][2 * r + e],
@@ -385,14 +427,14 @@ __global__ void __launch_bounds__(kThreads) cached_mma_kernel(const CachedArgs a
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float f = exp2f(jm[w][row] - base);
-      const float4 o = *reinterpret_cast<const float4*>(&jo[w][row][col]);
+      const float4 o = *reinterpret_cast<const float4*>(jo + (w * 16 + row) * (DP + 4) + col);
       sum[0] += f * o.x, sum[1] += f * o.y, sum[2] += f * o.z, sum[3] += f * o.w;
       ls += f * jl[w][row];
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) put<T>(a, row0 + row, blockIdx.x, col + e, sum[e], ls);
+    for (int e = 0; e < 4; ++e) put<T>(a, row0 + row, chunk, col + e, sum[e], ls);
     if (a.chunks > 1 && col == 0) {
-      float* st = part_stats(a) + ((row0 + row) * a.chunks + blockIdx.x) * 2;
+      float* st = part_stats(a) + ((row0 + row) * a.chunks + chunk) * 2;
       st[0] = mx;
       st[1] = ls;
     }
@@ -400,52 +442,76 @@ __global__ void __launch_bounds__(kThreads) cached_mma_kernel(const CachedArgs a
 }
 
 // Joins the chunks of a head's row: o = sum_c 2^(m_c - m) sum_c / sum_c 2^(m_c - m) l_c.
-// A block per row; eight strands of chunks, joined in order.
-template <typename T>
+// CL lanes of four columns, STRANDS of chunks per row (joined in order); what is left of
+// the block's 256 threads are further rows.  Few chunks: a warp per row.  Many: 32
+// strands for 32 columns, so that even one row keeps many loads in flight.
+template <typename T, int CL, int STRANDS>
 __global__ void __launch_bounds__(256) cached_join_kernel(const CachedArgs a) {
-  __shared__ float so[8][256 + 1];
-  __shared__ float red[8];
+  constexpr int TPR = CL * STRANDS, ROWS = 256 / TPR;
+  static_assert(TPR == 32 || TPR == 256, "a row is a warp or the block");
+  __shared__ float4 so[STRANDS > 1 ? STRANDS : 1][CL];
+  __shared__ float red[2][8];
   pdl_wait();
-  const int64_t row = blockIdx.x;
-  const int n = (int)(row / a.H);
-  const int64_t len = length_of(a, n);
+  const int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / TPR;
+  if (row >= (int64_t)a.N * a.H) return;  // whole warps; with one row per block, none
+  const int64_t len = length_of(a, (int)(row / a.H));
   const int used = (int)max64(1, (len + a.chunk - 1) / a.chunk);
-  const float* st = part_stats(a) + row * a.chunks * 2;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  const float2* st = reinterpret_cast<const float2*>(part_stats(a) + row * a.chunks * 2);
+  const int t = threadIdx.x % TPR, lane = threadIdx.x & 31, warp = threadIdx.x / 32;
   float mx = -INFINITY;
-  for (int c = threadIdx.x; c < used; c += 256) mx = fmaxf(mx, st[2 * c]);
+  for (int c = t; c < used; c += TPR) mx = fmaxf(mx, st[c].x);
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-  if (lane == 0) red[warp] = mx;
-  __syncthreads();
-  mx = red[0];
+  if (TPR > 32) {
+    if (lane == 0) red[0][warp] = mx;
+    __syncthreads();
 #pragma unroll
-  for (int w = 1; w < 8; ++w) mx = fmaxf(mx, red[w]);
-  const float base = mx == -INFINITY ? 0.f : mx;
-  float l = 0.f, acc[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-  for (int c = warp; c < used; c += 8) {
-    const float f = exp2f(st[2 * c] - base);
-    l += f * st[2 * c + 1];
-    const float* p = a.part + (row * a.chunks + c) * a.D;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < a.D) acc[i] = fmaf(f, p[lane + 32 * i], acc[i]);
+    for (int w = 0; w < 8; ++w) mx = fmaxf(mx, red[0][w]);
   }
+  const float base = mx == -INFINITY ? 0.f : mx;
+  float l = 0.f;
+  for (int c = t; c < used; c += TPR) l += exp2f(st[c].x - base) * st[c].y;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) so[warp][lane + 32 * i] = acc[i];
-  if (lane == 0) so[warp][256] = l;
-  __syncthreads();
-  const int c = threadIdx.x;
-  if (c < a.D) {
-    float s = 0.f, ls = 0.f;
+  for (int x = 16; x > 0; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+  if (TPR > 32) {
+    if (lane == 0) red[1][warp] = l;
+    __syncthreads();
+    l = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-      s += so[w][c];
-      ls += so[w][256];
+    for (int w = 0; w < 8; ++w) l += red[1][w];
+  }
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+  const int pitch = part_pitch(a.D), strand = t / CL;
+  for (int col = ((int)blockIdx.y * CL + t % CL) * 4; col - (t % CL) * 4 < a.D; col += (int)gridDim.y * CL * 4) {
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (col < a.D) {
+      const float* p = a.part + row * a.chunks * pitch + col;
+#pragma unroll 8
+      for (int c = strand; c < used; c += STRANDS) {
+        const float f = exp2f(st[c].x - base);
+        const float4 v = *reinterpret_cast<const float4*>(p + (int64_t)c * pitch);
+        s.x = fmaf(f, v.x, s.x), s.y = fmaf(f, v.y, s.y), s.z = fmaf(f, v.z, s.z), s.w = fmaf(f, v.w, s.w);
+      }
     }
-    ((T*)a.o)[row * a.D + c] = from_acc<T>(ls > 0.f ? s / ls : ls == 0.f ? 0.f : ls);
+    if (STRANDS > 1) {
+      __syncthreads();
+      so[strand][t % CL] = s;
+      __syncthreads();
+      if (strand == 0) {
+#pragma unroll 8
+        for (int i = 1; i < STRANDS; ++i) {
+          const float4 v = so[i][t];
+          s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+        }
+      }
+    }
+    if (strand == 0) {
+      T* o = (T*)a.o + row * a.D + col;
+      const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (col + e < a.D) o[e] = from_acc<T>(v[e] * inv);
+    }
   }
 }
 
@@ -453,15 +519,21 @@ __global__ void __launch_bounds__(256) cached_join_kernel(const CachedArgs a) {
 // host
 // ---------------------------------------------------------------------------
 
-// Tokens per chunk: a whole number of block steps (128 tokens), few enough that
-// the grid holds about eight blocks per SM, at least 128.
-int64_t chunk_tokens(int64_t N, int64_t Hk, int64_t P) {
-  const int64_t pairs = max64(1, N * Hk), target = 148 * 8;
-  const int64_t chunks = max64(1, min64((P + 127) / 128, (target + pairs - 1) / pairs));
-  return max64(128, ((P + chunks - 1) / chunks + 127) / 128 * 128);
+// Blocks that an SM holds: of the matrix kernel by its shared memory, of the other
+// by its registers (for the common widths).
+constexpr int kMmaBlocks = 3, kSimtBlocks = 8;
+
+// Tokens per chunk.  One cloud: as many chunks as blocks fit on the GPU at once.  Several: two such waves and at least five chunks each, since their lengths
+// are not known here and differ.  Splitting a short axis costs a join (about 4 us): with enough
+// blocks without it, not below 512 tokens.
+int64_t chunk_tokens(int64_t N, int64_t Hk, int64_t P, int per_sm) {
+  const int64_t pairs = max64(1, N * Hk), waves = 148 * per_sm, least = pairs < 148 ? 64 : 512;
+  const int64_t wish = N == 1 ? waves / pairs : max64(2 * waves / pairs, 5);
+  const int64_t chunks = max64(1, min64((P + least - 1) / least, wish));
+  return max64(64, ((P + chunks - 1) / chunks + 63) / 64 * 64);
 }
-int64_t chunk_count(int64_t N, int64_t Hk, int64_t P) {
-  const int64_t c = chunk_tokens(N, Hk, P);
+int64_t chunk_count(int64_t N, int64_t Hk, int64_t P, int per_sm) {
+  const int64_t c = chunk_tokens(N, Hk, P, per_sm);
   return max64(1, (P + c - 1) / c);
 }
 
@@ -469,7 +541,7 @@ template <typename T, int VEC, int LPK, int NVL, int GB>
 int simt_launch(const CachedArgs& a, cudaStream_t st) {
   const int gblocks = (a.H / a.Hk + GB - 1) / GB;
   cached_simt_kernel<T, VEC, LPK, NVL, GB>
-      <<<dim3(a.chunks, a.N, a.Hk * gblocks), kThreads, 0, st>>>(a);
+      <<<dim3(a.Hk * gblocks, a.chunks, a.N), kThreads, 0, st>>>(a);
   return check_launch();
 }
 template <typename T, int VEC, int LPK, int NVL>
@@ -488,24 +560,40 @@ bool aligned16(const CachedArgs& a) {
          (a.q_sn | a.q_sh | a.k_sn | a.k_sp | a.k_sh | a.v_sn | a.v_sp | a.v_sh) % V == 0;
 }
 
+// A warp per row while that leaves no long chain of chunks.
+template <typename T>
+int join_launch(const CachedArgs& a, cudaStream_t st) {
+  const int64_t rows = (int64_t)a.N * a.H;
+  if (a.chunks <= 8)
+    return launch_pdl(cached_join_kernel<T, 32, 1>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, a);
+  return launch_pdl(cached_join_kernel<T, 8, 32>, dim3((unsigned)rows, (a.D + 31) / 32), dim3(256), 0, st, a);
+}
+
 template <typename T, int DP>
 int mma_launch(const CachedArgs& a, cudaStream_t st) {
   const int group = a.H / a.Hk;
-  const dim3 grid(a.chunks, a.N, a.Hk * ((group + 15) / 16));
-  if (group > 8) cached_mma_kernel<T, DP, true><<<grid, kThreads, 0, st>>>(a);
-  else cached_mma_kernel<T, DP, false><<<grid, kThreads, 0, st>>>(a);
+  const dim3 grid(a.Hk * ((group + 15) / 16), a.chunks, a.N);  // neighbours read the same tokens' heads
+  auto kern = group > 8 ? cached_mma_kernel<T, DP, true> : cached_mma_kernel<T, DP, false>;
+  constexpr int smem = MmaShape<DP>::smem;
+  const int s = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (s) return s;
+  kern<<<grid, kThreads, smem, st>>>(a);
   return check_launch();
 }
 
 template <typename T>
-int cached_typed(const CachedArgs& a, cudaStream_t st) {
+int cached_typed(CachedArgs a, cudaStream_t st) {
   constexpr int V = 16 / sizeof(T);
+  const bool mma = sizeof(T) == 2 && a.D <= 128 && aligned16<T>(a);
+  const int per_sm = mma ? kMmaBlocks : kSimtBlocks;
+  a.chunk = chunk_tokens(a.N, a.Hk, a.P, per_sm);
+  a.chunks = (int)chunk_count(a.N, a.Hk, a.P, per_sm);
   int s;
   if constexpr (sizeof(T) == 2) {
-    if (a.D <= 128 && aligned16<T>(a)) {
+    if (mma) {
       s = a.D <= 64 ? mma_launch<T, 64>(a, st) : mma_launch<T, 128>(a, st);
       if (s || a.chunks == 1) return s;
-      return launch_pdl(cached_join_kernel<T>, dim3((unsigned)(a.N * a.H)), dim3(256), 0, st, a);
+      return join_launch<T>(a, st);
     }
   }
   if (aligned16<T>(a)) {
@@ -518,29 +606,29 @@ int cached_typed(const CachedArgs& a, cudaStream_t st) {
     else s = simt_group<T, 1, 32, 8>(a, st);
   }
   if (s || a.chunks == 1) return s;
-  return launch_pdl(cached_join_kernel<T>, dim3((unsigned)(a.N * a.H)), dim3(256), 0, st, a);
+  return join_launch<T>(a, st);
 }
 
 }  // namespace
 
 size_t cached_workspace_size(int64_t N, int64_t H, int64_t Hk, int64_t P, int64_t D) {
-  const int64_t chunks = chunk_count(N, Hk, P);
-  return chunks == 1 ? 0 : (size_t)(N * H) * chunks * (D + 2) * sizeof(float);
+  const int64_t chunks = max64(chunk_count(N, Hk, P, kMmaBlocks), chunk_count(N, Hk, P, kSimtBlocks));
+  return chunks == 1 ? 0 : (size_t)(N * H) * chunks * (part_pitch((int)D) + 2) * sizeof(float);
 }
 
 int cached_attention(int dtype, const void* q, const int64_t* q_stride, const void* k,
                      const int64_t* k_stride, const void* v, const int64_t* v_stride,
                      const int64_t* lengths, int64_t N, int64_t P, int64_t H, int64_t Hk, int64_t D,
                      float scale, void* o, void* ws, cudaStream_t st) {
-  CachedArgs a;
+  CachedArgs a = {};
   a.q = q, a.k = k, a.v = v;
   a.q_sn = q_stride[0], a.q_sh = q_stride[1];
   a.k_sn = k_stride[0], a.k_sp = k_stride[1], a.k_sh = k_stride[2];
   a.v_sn = v_stride[0], a.v_sp = v_stride[1], a.v_sh = v_stride[2];
   a.lengths = lengths;
   a.o = o, a.part = (float*)ws;
-  a.P = P, a.chunk = chunk_tokens(N, Hk, P);
-  a.N = (int)N, a.H = (int)H, a.Hk = (int)Hk, a.D = (int)D, a.chunks = (int)chunk_count(N, Hk, P);
+  a.P = P;
+  a.N = (int)N, a.H = (int)H, a.Hk = (int)Hk, a.D = (int)D;
   a.qscale = scale * kLog2e;
   switch (dtype) {
     case TPO_F32: return cached_typed<float>(a, st);

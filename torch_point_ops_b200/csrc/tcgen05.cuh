@@ -43,9 +43,12 @@ __device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, volatile
   atomicOr(err, kErrMmaTimeout);
 }
 
+#ifndef CPH
+#define CPH ""
+#endif
 // ---- 16-byte asynchronous copies; a false predicate writes zeros ----
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool read) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
+  asm volatile("cp.async.cg.shared.global" CPH " [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>

@@ -13,7 +13,7 @@
 //
 // Slots at or beyond lengths[n] are never read: they may hold anything.
 #include "attention_common.cuh"
-#include "tcgen05.cuh"  // pack2
+#include "tcgen05.cuh"  // asynchronous copies
 
 namespace tpo {
 namespace {

@@ -41,11 +41,52 @@ __device__ __forceinline__ A row_sum(A v, A* red, int bar) {
 template <typename A>
 __device__ __forceinline__ A inv_std(A var, A eps);
 template <>
-__device__ __forceinline__ float inv_std<float>(float var, float eps) { return 1.0f / sqrtf(var + eps); }
+__device__ __forceinline__ float inv_std<float>(float var, float eps) { return rsqrtf(var + eps); }  // within 2 ulp
 template <>
-__device__ __forceinline__ double inv_std<double>(double var, double eps) { return 1.0 / sqrt(var + eps); }
+__device__ __forceinline__ double inv_std<double>(double var, double eps) { return rsqrt(var + eps); }
+
+// A thread's vectors of a row (vector i: columns (i * TPR + t) * VEC on) as accumulators.
+// Vectors beyond column C are zeros: they are cleared once and never loaded, so no
+// element needs a test of its own.
+template <int VEC, int N, typename T, typename A>
+__device__ __forceinline__ void unpack(A (&v)[N * VEC], const Pack<T, VEC> (&raw)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if constexpr (VEC == 1) {
+      v[i] = to_acc(raw[i].v[0]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < VEC / 2; ++j) pair_of(raw[i], j, v[i * VEC + 2 * j], v[i * VEC + 2 * j + 1]);
+    }
+  }
+}
+template <int VEC, int TPR, int EPT, typename T>
+__device__ __forceinline__ void load_row(Pack<T, VEC> (&raw)[EPT / VEC], const T* row, int t, int C) {
+#pragma unroll
+  for (int i = 0; i < EPT / VEC; ++i) {
+    const int c = (i * TPR + t) * VEC;
+    if (c < C) raw[i] = *reinterpret_cast<const Pack<T, VEC>*>(row + c);
+  }
+}
+template <int VEC, int N, typename T>
+__device__ __forceinline__ void fill(Pack<T, VEC> (&raw)[N], Acc<T> value) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) raw[i].v[j] = from_acc<T>(value);
+}
+template <int VEC, int TPR, int EPT, typename T, typename A>
+__device__ __forceinline__ void store_row(T* row, const A (&v)[EPT], int t, int C) {
+#pragma unroll
+  for (int i = 0; i < EPT / VEC; ++i) {
+    const int c = (i * TPR + t) * VEC;
+    if (c < C) store_vec<VEC>(row + c, v + i * VEC);
+  }
+}
 
 // TPR threads per row, EPT elements per thread in vectors of VEC, RPB rows per block.
+// Blocks stay resident and walk over the rows: weight and bias are read once into
+// registers (with a block per row group they cost as many loads as the row itself).
 template <typename T, typename W, int VEC, int TPR, int EPT, int RPB>
 __global__ void __launch_bounds__(TPR* RPB)
     ln_fwd_kernel(const T* __restrict__ x, int64_t xs, const W* __restrict__ w,
@@ -53,36 +94,42 @@ __global__ void __launch_bounds__(TPR* RPB)
                   Acc<T>* __restrict__ mean_out, Acc<T>* __restrict__ rstd_out) {
   using A = Acc<T>;
   constexpr int NV = EPT / VEC;
+  // 32 and 64 bits: the next row is on its way while this one is reduced and written.
+  // 16 bits: conversions keep the issue slots busy, and the registers of a second
+  // row cost more warps than it brings (measured, 32768 x 1024: 30.7 against 29.7 us).
+  constexpr bool AHEAD = sizeof(T) != 2;
   __shared__ A red[RPB][4][TPR / 32];
   const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
   const A eps = (A)eps_, inv_c = (A)1 / (A)C;
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + g;
+  if (row >= rows) return;  // a whole row group: its barrier is its own
+  Pack<T, VEC> cur[NV], nxt[NV];
+  Pack<W, VEC> wv[NV], bv[NV];
+  fill(cur, 0);
+  fill(nxt, 0);
+  fill(wv, 1);  // no weight, no bias: one and zero, so that the loop has no branches
+  fill(bv, 0);
+  load_row<VEC, TPR, EPT>(cur, x + row * xs, t, C);
+  if (w) load_row<VEC, TPR, EPT>(wv, w, t, C);
+  if (b) load_row<VEC, TPR, EPT>(bv, b, t, C);
   int phase = 0;
-  for (int64_t row = (int64_t)blockIdx.x * RPB + g; row < rows; row += (int64_t)gridDim.x * RPB) {
-    const T* xr = x + row * xs;
-    A v[EPT];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + t) * VEC;
-      if (c < C) {
-        load_vec<VEC>(xr + c, v + i * VEC);
-      } else {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[i * VEC + j] = 0;
-      }
-    }
-    A s = 0;
+  while (row < rows) {
+    const int64_t next = row + step;
+    if (AHEAD && next < rows) load_row<VEC, TPR, EPT>(nxt, x + next * xs, t, C);
+    A v[EPT], s = 0;
+    unpack(v, cur);
 #pragma unroll
     for (int e = 0; e < EPT; ++e) s += v[e];
     const A mean = row_sum<TPR>(s, red[g][phase], g + 1) * inv_c;
     s = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if ((i * TPR + t) * VEC < C) {
+      const A m = (i * TPR + t) * VEC < C ? mean : (A)0;  // vectors beyond C are no part of the variance
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const A d = v[i * VEC + j] - mean;
-          s += d * d;
-        }
+      for (int j = 0; j < VEC; ++j) {
+        v[i * VEC + j] -= m;
+        s += v[i * VEC + j] * v[i * VEC + j];
       }
     }
     const A rstd = inv_std<A>(row_sum<TPR>(s, red[g][phase + 1], g + 1) * inv_c, eps);
@@ -91,21 +138,23 @@ __global__ void __launch_bounds__(TPR* RPB)
       mean_out[row] = mean;
       rstd_out[row] = rstd;
     }
-    T* yr = y + row * C;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + t) * VEC;
-      if (c < C) {
-        A o[VEC], wv[VEC], bv[VEC];
+      A o[VEC], wk[VEC], bk[VEC];
+      unpack<VEC, 1>(wk, reinterpret_cast<const Pack<W, VEC>(&)[1]>(wv[i]));
+      unpack<VEC, 1>(bk, reinterpret_cast<const Pack<W, VEC>(&)[1]>(bv[i]));
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) wv[j] = 1, bv[j] = 0;
-        if (w) load_vec<VEC>(w + c, wv);
-        if (b) load_vec<VEC>(b + c, bv);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) o[j] = (v[i * VEC + j] - mean) * rstd * wv[j] + bv[j];
-        store_vec<VEC>(yr + c, o);
-      }
+      for (int j = 0; j < VEC; ++j) o[j] = v[i * VEC + j] * rstd * wk[j] + bk[j];
+      if (c < C) store_vec<VEC>(y + row * C + c, o);
     }
+    if (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) cur[i] = nxt[i];
+    } else if (next < rows) {
+      load_row<VEC, TPR, EPT>(cur, x + next * xs, t, C);
+    }
+    row = next;
   }
 }
 
@@ -115,7 +164,7 @@ __global__ void __launch_bounds__(TPR* RPB)
 // of each (summed by ln_bwd_reduce_kernel in block order: no atomics, the same
 // bits in every run).
 template <typename T, typename W, int VEC, int TPR, int EPT, int RPB>
-__global__ void __launch_bounds__(TPR* RPB)
+__global__ void __launch_bounds__(TPR* RPB, TPR* RPB <= 256 ? 2 : 1)
     ln_bwd_kernel(const T* __restrict__ x, int64_t xs, const T* __restrict__ dy, int64_t dys,
                   const W* __restrict__ w, const Acc<T>* __restrict__ mean_in,
                   const Acc<T>* __restrict__ rstd_in, int64_t rows, int C, T* __restrict__ dx,
@@ -126,42 +175,49 @@ __global__ void __launch_bounds__(TPR* RPB)
   __shared__ A comb[RPB > 1 ? 2 * TPR * EPT : 1];
   const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
   const A inv_c = (A)1 / (A)C;
-  A wv[EPT], aw[EPT], ab[EPT];
+  A aw[EPT], ab[EPT];
 #pragma unroll
-  for (int e = 0; e < EPT; ++e) wv[e] = 1, aw[e] = 0, ab[e] = 0;
-  if (w) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + t) * VEC;
-      if (c < C) load_vec<VEC>(w + c, wv + i * VEC);
-    }
-  }
+  for (int e = 0; e < EPT; ++e) aw[e] = ab[e] = 0;
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t row = (int64_t)blockIdx.x * RPB + g;
+  Pack<T, VEC> cx[NV], cy[NV];
+  Pack<W, VEC> wv[NV];
+  fill(cx, 0);
+  fill(cy, 0);
+  fill(wv, 1);
+  A mean = 0, rstd = 0;
+  auto fetch = [&](int64_t r) {
+    load_row<VEC, TPR, EPT>(cx, x + r * xs, t, C);
+    load_row<VEC, TPR, EPT>(cy, dy + r * dys, t, C);
+    mean = mean_in[r], rstd = rstd_in[r];
+  };
+  // 16-bit rows: the next one is on its way while this one is reduced and written.
+  // Wider types have as many bytes in flight without it, and no registers for it.
+  constexpr bool AHEAD = sizeof(T) == 2;
+  if (AHEAD && row < rows) fetch(row);
+  if (w) load_row<VEC, TPR, EPT>(wv, w, t, C);
   int phase = 0;
-  for (int64_t row = (int64_t)blockIdx.x * RPB + g; row < rows; row += (int64_t)gridDim.x * RPB) {
-    A xh[EPT], gy[EPT];
+  for (; row < rows; row += step) {
+    if (!AHEAD) fetch(row);
+    const A m = mean, r = rstd;
+    A xh[EPT], u[EPT], s1 = 0, s2 = 0;
+    unpack(xh, cx);
+    unpack(u, cy);
+    if (AHEAD && row + step < rows) fetch(row + step);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + t) * VEC;
-      if (c < C) {
-        load_vec<VEC>(x + row * xs + c, xh + i * VEC);
-        load_vec<VEC>(dy + row * dys + c, gy + i * VEC);
-      }
-    }
-    const A mean = mean_in[row], rstd = rstd_in[row];
-    A s1 = 0, s2 = 0;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const bool in = (i * TPR + t) * VEC < C;
+      A wk[VEC];
+      unpack<VEC, 1>(wk, reinterpret_cast<const Pack<W, VEC>(&)[1]>(wv[i]));
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
+        // beyond column C dy is zero, so whatever xh is there adds nothing
         const int e = i * VEC + j;
-        xh[e] = in ? (xh[e] - mean) * rstd : 0;
-        gy[e] = in ? gy[e] : 0;
-        aw[e] += gy[e] * xh[e];
-        ab[e] += gy[e];
-        const A u = gy[e] * wv[e];
-        s1 += u;
-        s2 += u * xh[e];
+        xh[e] = (xh[e] - m) * r;
+        aw[e] += u[e] * xh[e];
+        ab[e] += u[e];
+        u[e] *= wk[j];
+        s1 += u[e];
+        s2 += u[e] * xh[e];
       }
     }
     if (dx) {
@@ -169,18 +225,8 @@ __global__ void __launch_bounds__(TPR* RPB)
       s2 = row_sum<TPR>(s2, red[g][phase + 1], g + 1) * inv_c;
       phase ^= 2;
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = (i * TPR + t) * VEC;
-        if (c < C) {
-          A o[VEC];
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const int e = i * VEC + j;
-            o[j] = rstd * (gy[e] * wv[e] - s1 - xh[e] * s2);
-          }
-          store_vec<VEC>(dx + row * C + c, o);
-        }
-      }
+      for (int e = 0; e < EPT; ++e) u[e] = r * (u[e] - s1 - xh[e] * s2);
+      store_row<VEC, TPR, EPT>(dx + row * C, u, t, C);
     }
   }
   if (!pw && !pb) return;
@@ -204,41 +250,34 @@ __global__ void __launch_bounds__(TPR* RPB)
     __syncthreads();
   }
   if (g == 0) {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        const int c = (i * TPR + t) * VEC + j;
-        if (c < C) {
-          if (pw) pw[(int64_t)blockIdx.x * C + c] = aw[i * VEC + j];
-          if (pb) pb[(int64_t)blockIdx.x * C + c] = ab[i * VEC + j];
-        }
-      }
-    }
+    if (pw) store_row<VEC, TPR, EPT>(pw + (int64_t)blockIdx.x * C, aw, t, C);
+    if (pb) store_row<VEC, TPR, EPT>(pb + (int64_t)blockIdx.x * C, ab, t, C);
   }
 }
 
-// Column sums of the blocks' partial rows: 32 columns per block, 32 strands of
+// Column sums of the blocks' partial rows: 32 columns per block, STRANDS strands of
 // rows each, strands added in order.  blockIdx.y 0: weight, 1: bias.
-template <typename W, typename A>
-__global__ void __launch_bounds__(1024)
+template <typename W, typename A, int STRANDS>
+__global__ void __launch_bounds__(32 * STRANDS)
     ln_bwd_reduce_kernel(const A* __restrict__ pw, const A* __restrict__ pb, int parts, int C,
                          W* __restrict__ dw, W* __restrict__ db) {
-  __shared__ A sm[32][33];
+  __shared__ A sm[STRANDS][33];
   pdl_wait();
   const A* p = blockIdx.y ? pb : pw;
   W* out = blockIdx.y ? db : dw;
   if (!out) return;
   const int c = blockIdx.x * 32 + threadIdx.x;
   A s = 0;
-  if (c < C)
-    for (int r = threadIdx.y; r < parts; r += 32) s += p[(int64_t)r * C + c];
+  if (c < C) {
+#pragma unroll 8
+    for (int r = threadIdx.y; r < parts; r += STRANDS) s += p[(int64_t)r * C + c];
+  }
   sm[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.y == 0 && c < C) {
     s = 0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) s += sm[i][threadIdx.x];
+    for (int i = 0; i < STRANDS; ++i) s += sm[i][threadIdx.x];
     out[c] = from_acc<W>(s);
   }
 }
@@ -327,67 +366,86 @@ __global__ void __launch_bounds__(256)
   if (pb) pb[(int64_t)blockIdx.y * C + c] = ab;
 }
 
-// Resident blocks of the backward kernel: two per SM.
+// Blocks of the backward kernel: two per SM.
 constexpr int kBwdBlocks = 148 * 2;
 constexpr int kWideParts = 32;
 
-int bwd_parts(int64_t rows, int64_t C) {
-  if (C > kMaxRegWidth) return (int)min64(rows, kWideParts);
-  const int rpb = C <= 512 ? 8 : C <= 1024 ? 4 : C <= 2048 ? 2 : 1;
-  return (int)min64((rows + rpb - 1) / rpb, kBwdBlocks);
+// Rows per block of the backward kernel.  Whole 16-byte vectors: 16 elements per
+// thread; else 8, so that the narrow loads spread over more warps.
+int bwd_rows_per_block(int64_t C, bool vec) {
+  if (vec) return C <= 512 ? 8 : C <= 1024 ? 4 : C <= 2048 ? 2 : 1;
+  return C <= 256 ? 8 : C <= 512 ? 4 : C <= 1024 ? 2 : 1;
+}
+int bwd_parts(int64_t rows, int64_t C, int rpb) {
+  return (int)min64((rows + rpb - 1) / rpb, C > kMaxRegWidth ? kWideParts : kBwdBlocks);
+}
+
+template <typename K>
+int resident_blocks(K kern, int threads) {
+  int n = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != cudaSuccess || n < 1) n = 1;
+  return 148 * n;
 }
 
 template <typename T, typename W, int VEC>
 int fwd_launch(const T* x, int64_t xs, const W* w, const W* b, int64_t rows, int C, double eps, T* y,
                Acc<T>* mean, Acc<T>* rstd, cudaStream_t st) {
-  constexpr int64_t kMaxGrid = (int64_t(1) << 31) - 1;
-#define TPO_LN(TPR, EPT, RPB)                                                                   \
-  do {                                                                                          \
-    const int64_t grid = min64((rows + RPB - 1) / RPB, kMaxGrid);                               \
-    ln_fwd_kernel<T, W, VEC, TPR, EPT, RPB>                                                     \
-        <<<(unsigned)grid, TPR * RPB, 0, st>>>(x, xs, w, b, rows, C, eps, y, mean, rstd);       \
-    return check_launch();                                                                      \
+#define TPO_LN(TPR, EPT, RPB)                                                                          \
+  do {                                                                                                 \
+    auto kern = ln_fwd_kernel<T, W, VEC, TPR, EPT, RPB>;                                               \
+    static const int most = resident_blocks(kern, TPR * RPB);                                          \
+    kern<<<(unsigned)min64((rows + RPB - 1) / RPB, most), TPR * RPB, 0, st>>>(x, xs, w, b, rows, C,    \
+                                                                              eps, y, mean, rstd);     \
+    return check_launch();                                                                             \
   } while (0)
-  // A warp per row up to 1024 columns (no block barrier), four rows per block;
-  // one block per row beyond.
   if (C <= 256) TPO_LN(32, 8, 4);
-  if (C <= 512) TPO_LN(32, 16, 4);
-  if (C <= 1024) TPO_LN(32, 32, 4);
-  if (C <= 2048) TPO_LN(128, 16, 1);
-  if (C <= 4096) TPO_LN(128, 32, 1);
-  TPO_LN(256, 32, 1);
+  if constexpr (VEC * sizeof(T) == 16) {  // a warp per row up to 1024 columns: no barrier
+    if (C <= 512) TPO_LN(32, 16, 4);
+    if (C <= 1024) TPO_LN(32, 32, 4);
+    if (C <= 2048) TPO_LN(128, 16, 1);
+    if (C <= 4096) TPO_LN(128, 32, 1);
+    TPO_LN(256, 32, 1);
+  } else {  // narrow loads: 8 elements per thread, more warps
+    if (C <= 512) TPO_LN(64, 8, 2);
+    if (C <= 1024) TPO_LN(128, 8, 1);
+    if (C <= 2048) TPO_LN(256, 8, 1);
+    if (C <= 4096) TPO_LN(512, 8, 1);
+    TPO_LN(512, 16, 1);
+  }
 #undef TPO_LN
 }
 
 template <typename T, typename W, int VEC>
 int bwd_launch(const T* x, int64_t xs, const T* dy, int64_t dys, const W* w, const Acc<T>* mean,
-               const Acc<T>* rstd, int64_t rows, int C, T* dx, Acc<T>* pw, Acc<T>* pb,
+               const Acc<T>* rstd, int64_t rows, int C, int grid, T* dx, Acc<T>* pw, Acc<T>* pb,
                cudaStream_t st) {
-  const int grid = bwd_parts(rows, C);
-#define TPO_LN(TPR, RPB)                                                                        \
+#define TPO_LN(TPR, EPT, RPB)                                                                   \
   do {                                                                                          \
-    ln_bwd_kernel<T, W, VEC, TPR, C16(TPR), RPB><<<grid, TPR * RPB, 0, st>>>(                   \
+    ln_bwd_kernel<T, W, VEC, TPR, EPT, RPB><<<grid, TPR * RPB, 0, st>>>(                        \
         x, xs, dy, dys, w, mean, rstd, rows, C, dx, pw, pb);                                    \
     return check_launch();                                                                      \
   } while (0)
-#define C16(TPR) 16
-  if (C <= 256) {
-    ln_bwd_kernel<T, W, VEC, 32, 8, 8>
-        <<<grid, 256, 0, st>>>(x, xs, dy, dys, w, mean, rstd, rows, C, dx, pw, pb);
-    return check_launch();
+  if (C <= 256) TPO_LN(32, 8, 8);
+  if constexpr (VEC * sizeof(T) == 16) {
+    if (C <= 512) TPO_LN(32, 16, 8);
+    if (C <= 1024) TPO_LN(64, 16, 4);
+    if (C <= 2048) TPO_LN(128, 16, 2);
+    if (C <= 4096) TPO_LN(256, 16, 1);
+  } else {
+    if (C <= 512) TPO_LN(64, 8, 4);
+    if (C <= 1024) TPO_LN(128, 8, 2);
+    if (C <= 2048) TPO_LN(256, 8, 1);
+    if (C <= 4096) TPO_LN(512, 8, 1);
   }
-  if (C <= 512) TPO_LN(32, 8);
-  if (C <= 1024) TPO_LN(64, 4);
-  if (C <= 2048) TPO_LN(128, 2);
-  if (C <= 4096) TPO_LN(256, 1);
-  TPO_LN(512, 1);
-#undef C16
+  TPO_LN(512, 16, 1);
 #undef TPO_LN
 }
 
-template <typename T>
+// Whether vectors of V elements (at most 16 bytes of alignment) may be read from rows of p.
+template <typename T, int V>
 bool vec_ok(const void* p, int64_t stride) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (stride * (int64_t)sizeof(T)) % 16 == 0;
+  constexpr size_t bytes = alignof(Pack<T, V>);
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0 && stride % V == 0;
 }
 
 template <typename T, typename W>
@@ -403,8 +461,13 @@ int fwd_typed(const void* x_, int64_t xs, const void* w_, const void* b_, int64_
                                                                           mean, rstd);
     return check_launch();
   }
-  // 16-byte accesses where every row and the parameters start on 16 bytes
-  const bool vec = vec_ok<T>(x, xs) && vec_ok<T>(y, C) && vec_ok<W>(w, 0) && vec_ok<W>(b, 0) && C % V == 0;
+  // 16-byte accesses where every row and the parameters start on 16 bytes; pairs of
+  // 16-bit elements where they start on whole pairs; else single elements
+  const bool vec = vec_ok<T, V>(x, xs) && vec_ok<T, V>(y, C) && vec_ok<W, V>(w, 0) && vec_ok<W, V>(b, 0) && C % V == 0;
+  if constexpr (V == 8) {
+    if (!vec && vec_ok<T, 2>(x, xs) && vec_ok<T, 2>(y, C) && vec_ok<W, 2>(w, 0) && vec_ok<W, 2>(b, 0) && C % 2 == 0)
+      return fwd_launch<T, W, 2>(x, xs, w, b, rows, (int)C, eps, y, mean, rstd, st);
+  }
   return vec ? fwd_launch<T, W, V>(x, xs, w, b, rows, (int)C, eps, y, mean, rstd, st)
              : fwd_launch<T, W, 1>(x, xs, w, b, rows, (int)C, eps, y, mean, rstd, st);
 }
@@ -419,10 +482,14 @@ int bwd_typed(const void* x_, int64_t xs, const void* dy_, int64_t dys, const vo
   const A *mean = (const A*)mean_, *rstd = (const A*)rstd_;
   T* dx = (T*)dx_;
   W *dw = (W*)dw_, *db = (W*)db_;
-  const int parts = bwd_parts(rows, C);
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = vec_ok<T, V>(x, xs) && vec_ok<T, V>(dy, dys) && vec_ok<T, V>(dx, C) && vec_ok<W, V>(w, 0) && C % V == 0;
+  const bool pairs = V == 8 && !vec && vec_ok<T, 2>(x, xs) && vec_ok<T, 2>(dy, dys) && vec_ok<T, 2>(dx, C) &&
+                     vec_ok<W, 2>(w, 0) && C % 2 == 0;
+  const int parts = bwd_parts(rows, C, C > kMaxRegWidth ? 1 : bwd_rows_per_block(C, vec));
   A* pw = dw ? (A*)ws : nullptr;
   A* pb = db ? (A*)ws + (int64_t)parts * C : nullptr;
-  int s;
+  int s = TPO_OK;
   if (C > kMaxRegWidth) {
     if (dx) {
       ln_bwd_wide_kernel<T, W><<<(unsigned)min64(rows, 148 * 4), 512, 0, st>>>(x, xs, dy, dys, w, mean, rstd,
@@ -435,21 +502,25 @@ int bwd_typed(const void* x_, int64_t xs, const void* dy_, int64_t dys, const vo
       if ((s = check_launch())) return s;
     }
   } else {
-    constexpr int V = 16 / sizeof(T);
-    const bool vec = vec_ok<T>(x, xs) && vec_ok<T>(dy, dys) && vec_ok<T>(dx, C) && vec_ok<W>(w, 0) && C % V == 0;
-    s = vec ? bwd_launch<T, W, V>(x, xs, dy, dys, w, mean, rstd, rows, (int)C, dx, pw, pb, st)
-            : bwd_launch<T, W, 1>(x, xs, dy, dys, w, mean, rstd, rows, (int)C, dx, pw, pb, st);
+    if constexpr (V == 8) {
+      if (pairs) s = bwd_launch<T, W, 2>(x, xs, dy, dys, w, mean, rstd, rows, (int)C, parts, dx, pw, pb, st);
+    }
+    if (!pairs) s = vec ? bwd_launch<T, W, V>(x, xs, dy, dys, w, mean, rstd, rows, (int)C, parts, dx, pw, pb, st)
+                        : bwd_launch<T, W, 1>(x, xs, dy, dys, w, mean, rstd, rows, (int)C, parts, dx, pw, pb, st);
     if (s) return s;
   }
   if (!dw && !db) return TPO_OK;
-  return launch_pdl(ln_bwd_reduce_kernel<W, A>, dim3((unsigned)((C + 31) / 32), 2), dim3(32, 32), 0, st,
-                    (const A*)pw, (const A*)pb, parts, (int)C, dw, db);
+  // many columns fill the GPU with short strands, few need the long ones' parallel loads
+  const dim3 grid((unsigned)((C + 31) / 32), 2);
+  if (parts <= 32 || C >= 2048)
+    return launch_pdl(ln_bwd_reduce_kernel<W, A, 8>, grid, dim3(32, 8), 0, st, (const A*)pw, (const A*)pb, parts, (int)C, dw, db);
+  return launch_pdl(ln_bwd_reduce_kernel<W, A, 32>, grid, dim3(32, 32), 0, st, (const A*)pw, (const A*)pb, parts, (int)C, dw, db);
 }
 
 }  // namespace
 
 size_t layer_norm_bwd_workspace_size(int dtype, int64_t rows, int64_t C) {
-  return (size_t)2 * bwd_parts(rows, C) * (size_t)C * (dtype == TPO_F64 ? 8 : 4);
+  return (size_t)2 * bwd_parts(rows, C, 1) * (size_t)C * (dtype == TPO_F64 ? 8 : 4);
 }
 
 #define TPO_LN_TYPES(CALL)                                                                  \

@@ -12,11 +12,14 @@
 // tiles (dK, dV), one owns query tiles (dQ), so nothing is added by atomics and
 // every run gives the same bits, at 7 products in place of 5.
 //
-// 256 threads as 16 x 16; a thread holds RM rows (ty) x CN columns (tx + 16 c) of
-// a score tile and RM rows x DP/16 columns of an output tile.  Both products read
-// four elements of the summed dimension per 16-byte shared-memory load: rows are
-// broadcast, columns sit in rows of DP + 4 floats (two wavefronts per load, no
-// bank conflicts), which gives 32 FMA cycles per 16 load cycles at RM = 8.
+// 256 threads as 16 x 16; thread (ty, tx) holds rows ty + 16 r (r < RM) x columns
+// tx + 16 c (c < CN) of a score tile and the same rows x DP/16 columns of an output
+// tile.  All products are packed fp32 FMAs, which hold the FP32 pipe for two cycles
+// and leave every other issue slot to loads: scores pair neighbouring elements of
+// the summed dimension (both come as pairs out of 16-byte loads), outputs pair rows
+// (the probabilities are kept transposed, a thread's rows side by side).  Rows of
+// operand tiles have DP + 4 floats: the 16 lanes of a column load touch every bank
+// twice, a row load is a broadcast of two rows in different banks.
 #include "attention_common.cuh"
 
 namespace tpo {
@@ -49,67 +52,126 @@ __device__ __forceinline__ void load_tile(float* dst, const T* src, int64_t stri
   }
 }
 
-// s[r][c] = sum_d a[ty*RM + r][d] * b[tx + 16c][d]
+// s[r][c] = sum_d a[ty + 16r][d] * b[tx + 16c][d]
 template <int DP, int RM, int CN>
 __device__ __forceinline__ void product_nt(float (&s)[RM][CN], const float* a, const float* b, int ty,
                                            int tx) {
+  constexpr int LD = DP + 4;
+  u64 acc[RM][CN];
 #pragma unroll
   for (int r = 0; r < RM; ++r)
 #pragma unroll
-    for (int c = 0; c < CN; ++c) s[r][c] = 0.f;
-  const float* ar = a + ty * RM * (DP + 4);
-  const float* br = b + tx * (DP + 4);
+    for (int c = 0; c < CN; ++c) acc[r][c] = 0;  // two zeros
+  const float* ar = a + ty * LD;
+  const float* br = b + tx * LD;
 #pragma unroll 2
   for (int d = 0; d < DP; d += 4) {
-    float4 bv[CN];
+    ulonglong2 bv[CN];
 #pragma unroll
-    for (int c = 0; c < CN; ++c) bv[c] = *reinterpret_cast<const float4*>(br + c * 16 * (DP + 4) + d);
+    for (int c = 0; c < CN; ++c) bv[c] = *reinterpret_cast<const ulonglong2*>(br + c * 16 * LD + d);
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
-      const float4 av = *reinterpret_cast<const float4*>(ar + r * (DP + 4) + d);
+      const ulonglong2 av = *reinterpret_cast<const ulonglong2*>(ar + r * 16 * LD + d);
 #pragma unroll
       for (int c = 0; c < CN; ++c) {
-        s[r][c] = fmaf(av.x, bv[c].x, s[r][c]);
-        s[r][c] = fmaf(av.y, bv[c].y, s[r][c]);
-        s[r][c] = fmaf(av.z, bv[c].z, s[r][c]);
-        s[r][c] = fmaf(av.w, bv[c].w, s[r][c]);
+        acc[r][c] = fma2(av.x, bv[c].x, acc[r][c]);
+        acc[r][c] = fma2(av.y, bv[c].y, acc[r][c]);
       }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < RM; ++r)
+#pragma unroll
+    for (int c = 0; c < CN; ++c) {
+      float x, y;
+      upk(acc[r][c], x, y);
+      s[r][c] = x + y;
+    }
+}
+
+// A thread's column j of a score-shaped tile, rows side by side, into p[j][ty*RM...].
+template <int BM, int RM>
+__device__ __forceinline__ void put_rows(float* p, int j, int ty, const float (&v)[RM]) {
+  float* at = p + j * (BM + 4) + ty * RM;
+  if constexpr (RM % 4 == 0) {
+#pragma unroll
+    for (int r = 0; r < RM; r += 4) *reinterpret_cast<float4*>(at + r) = make_float4(v[r], v[r + 1], v[r + 2], v[r + 3]);
+  } else {
+#pragma unroll
+    for (int r = 0; r < RM; r += 2) *reinterpret_cast<float2*>(at + r) = make_float2(v[r], v[r + 1]);
+  }
+}
+
+// o[rp][4g + i] += sum_j (p[j][ty*RM + 2rp], p[j][ty*RM + 2rp + 1]) * v[j][tx*4 + 64g + i]
+template <int DP, int RM, int BN>
+__device__ __forceinline__ void product_nn(u64 (&o)[RM / 2][DP / 16], const float* p, const float* v,
+                                           int ty, int tx) {
+  constexpr int LDP = 16 * RM + 4;
+  const float* pr = p + ty * RM;
+  const float* vr = v + tx * 4;
+#pragma unroll 4
+  for (int j = 0; j < BN; ++j) {
+    u64 pv[RM / 2];
+    if constexpr (RM % 4 == 0) {
+#pragma unroll
+      for (int r = 0; r < RM / 4; ++r) {
+        const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(pr + j * LDP + 4 * r);
+        pv[2 * r] = t.x, pv[2 * r + 1] = t.y;
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < RM / 2; ++r) pv[r] = *reinterpret_cast<const u64*>(pr + j * LDP + 2 * r);
+    }
+#pragma unroll
+    for (int g = 0; g < DP / 64; ++g) {
+      const float4 t = *reinterpret_cast<const float4*>(vr + j * (DP + 4) + g * 64);
+      const u64 vv[4] = {pk(t.x, t.x), pk(t.y, t.y), pk(t.z, t.z), pk(t.w, t.w)};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int r = 0; r < RM / 2; ++r) o[r][g * 4 + i] = fma2(pv[r], vv[i], o[r][g * 4 + i]);
     }
   }
 }
 
-// o[r][4g + i] += sum_j p[ty*RM + r][j] * v[j][tx*4 + 64g + i]
-template <int DP, int RM, int BN>
-__device__ __forceinline__ void product_nn(float (&o)[RM][DP / 16], const float* p, const float* v,
-                                           int ty, int tx) {
-  const float* pr = p + ty * RM * (BN + 4);
-#pragma unroll 1
-  for (int j = 0; j < BN; j += 4) {
-    float4 pv[RM];
+// The thread's part of a tile on its way from global to shared memory: requested early
+// (get), written where the buffer is free (put).
+template <typename T, int VEC, int DP, int ROWS>
+struct InFlight {
+  static constexpr int PER_ROW = DP / VEC, N = ROWS * PER_ROW / kThreads;
+  Pack<T, VEC> v[N];
+  __device__ __forceinline__ void get(const T* src, int64_t stride, int64_t valid, int D) {
 #pragma unroll
-    for (int r = 0; r < RM; ++r) pv[r] = *reinterpret_cast<const float4*>(pr + r * (BN + 4) + j);
+    for (int i = 0; i < N; ++i) {
+      const int at = threadIdx.x + i * kThreads, r = at / PER_ROW, c = (at % PER_ROW) * VEC;
 #pragma unroll
-    for (int jj = 0; jj < 4; ++jj) {
+      for (int j = 0; j < VEC; ++j) v[i].v[j] = from_acc<T>(0.f);
+      if (r < valid && c < D) v[i] = *reinterpret_cast<const Pack<T, VEC>*>(src + r * stride + c);
+    }
+  }
+  __device__ __forceinline__ void put(float* dst) const {
 #pragma unroll
-      for (int g = 0; g < DP / 64; ++g) {
-        const float4 vv = *reinterpret_cast<const float4*>(v + (j + jj) * (DP + 4) + tx * 4 + g * 64);
+    for (int i = 0; i < N; ++i) {
+      const int at = threadIdx.x + i * kThreads, r = at / PER_ROW, c = (at % PER_ROW) * VEC;
+      float f[VEC];
 #pragma unroll
-        for (int r = 0; r < RM; ++r) {
-          const float w = jj == 0 ? pv[r].x : jj == 1 ? pv[r].y : jj == 2 ? pv[r].z : pv[r].w;
-          o[r][g * 4 + 0] = fmaf(w, vv.x, o[r][g * 4 + 0]);
-          o[r][g * 4 + 1] = fmaf(w, vv.y, o[r][g * 4 + 1]);
-          o[r][g * 4 + 2] = fmaf(w, vv.z, o[r][g * 4 + 2]);
-          o[r][g * 4 + 3] = fmaf(w, vv.w, o[r][g * 4 + 3]);
-        }
+      for (int j = 0; j < VEC; ++j) f[j] = to_acc(v[i].v[j]);
+      float* d = dst + r * (DP + 4) + c;
+      if constexpr (VEC % 4 == 0) {
+#pragma unroll
+        for (int j = 0; j < VEC; j += 4) *reinterpret_cast<float4*>(d + j) = make_float4(f[j], f[j + 1], f[j + 2], f[j + 3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) d[j] = f[j];
       }
     }
   }
-}
+};
 
 template <int DP, int RM>
 struct FwdShape {
   static constexpr int BM = 16 * RM, BN = 64;
-  static constexpr int smem = ((BM + BN) * (DP + 4) + BM * (BN + 4)) * 4;
+  static constexpr int smem = ((BM + 2 * BN) * (DP + 4) + BN * (BM + 4)) * 4;
 };
 
 template <typename T, int VEC, int DP, int RM>
@@ -118,8 +180,9 @@ __global__ void __launch_bounds__(kThreads) packed_simt_fwd_kernel(const PackedA
   constexpr int BM = Sh::BM, BN = Sh::BN, CN = 4;
   extern __shared__ float4 smem4[];
   float* qs = reinterpret_cast<float*>(smem4);
-  float* kv = qs + BM * (DP + 4);
-  float* ps = kv + BN * (DP + 4);
+  float* ks = qs + BM * (DP + 4);
+  float* vs = ks + BN * (DP + 4);
+  float* ps = vs + BN * (DP + 4);
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   const int head = blockIdx.y, kvh = head / (a.H / a.Hk);
   // causal rows late in a cloud see most keys: those blocks start first
@@ -132,30 +195,34 @@ __global__ void __launch_bounds__(kThreads) packed_simt_fwd_kernel(const PackedA
   if (a.causal) nk = min64(nk, max64(first + t.rows + shift, 0));
   const float qscale = a.scale * kLog2e;
 
-  load_tile<T, VEC, DP>(qs, (const T*)a.q + t.row0 * a.q_st + head * a.q_sh, a.q_st, BM, t.rows, a.D);
   const T* kp = (const T*)a.k + t.b0 * a.k_st + kvh * a.k_sh;
   const T* vp = (const T*)a.v + t.b0 * a.v_st + kvh * a.v_sh;
-  float o[RM][DP / 16], m[RM], l[RM];
+  InFlight<T, VEC, DP, BN> next;
+  if (nk > 0) next.get(kp, a.k_st, nk, a.D);
+  load_tile<T, VEC, DP>(qs, (const T*)a.q + t.row0 * a.q_st + head * a.q_sh, a.q_st, BM, t.rows, a.D);
+  u64 o[RM / 2][DP / 16];
+  float m[RM], l[RM];
 #pragma unroll
   for (int r = 0; r < RM; ++r) {
     m[r] = -INFINITY;
     l[r] = 0.f;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) o[r][c] = 0.f;
+    for (int c = 0; c < DP / 16; ++c) o[r / 2][c] = 0;
   }
   for (int64_t j0 = 0; j0 < nk; j0 += BN) {
     const int valid = (int)min64(nk - j0, BN);
-    __syncthreads();
-    load_tile<T, VEC, DP>(kv, kp + j0 * a.k_st, a.k_st, BN, valid, a.D);
+    next.put(ks);  // the last readers of ks have passed the barrier before this step's P V
+    next.get(vp + j0 * a.v_st, a.v_st, nk - j0, a.D);
     __syncthreads();
     float s[RM][CN];
-    product_nt<DP, RM, CN>(s, qs, kv, ty, tx);
-    __syncthreads();
-    load_tile<T, VEC, DP>(kv, vp + j0 * a.v_st, a.v_st, BN, valid, a.D);
+    product_nt<DP, RM, CN>(s, qs, ks, ty, tx);
+    next.put(vs);  // the last P V is over: every thread has passed the barrier above since
+    if (j0 + BN < nk) next.get(kp + (j0 + BN) * a.k_st, a.k_st, nk - j0 - BN, a.D);
+    float corr[RM];
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
       int64_t lim = valid;
-      if (a.causal) lim = min64(lim, first + ty * RM + r + shift + 1 - j0);
+      if (a.causal) lim = min64(lim, first + ty + 16 * r + shift + 1 - j0);
       float mx = m[r];
 #pragma unroll
       for (int c = 0; c < CN; ++c) {
@@ -165,28 +232,38 @@ __global__ void __launch_bounds__(kThreads) packed_simt_fwd_kernel(const PackedA
 #pragma unroll
       for (int x = 8; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
       const float base = mx == -INFINITY ? 0.f : mx;  // a row that has seen nothing yet
-      const float corr = exp2f(m[r] - base);
+      corr[r] = exp2f(m[r] - base);
       float sum = 0.f;
 #pragma unroll
       for (int c = 0; c < CN; ++c) {
-        const float p = exp2f(s[r][c] - base);
-        sum += p;
-        ps[(ty * RM + r) * (BN + 4) + tx + 16 * c] = p;
+        s[r][c] = exp2f(s[r][c] - base);
+        sum += s[r][c];
       }
       m[r] = mx;
-      l[r] = l[r] * corr + sum;
+      l[r] = l[r] * corr[r] + sum;
+    }
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) o[r][c] *= corr;
+    for (int c = 0; c < CN; ++c) {
+      float col[RM];
+#pragma unroll
+      for (int r = 0; r < RM; ++r) col[r] = s[r][c];
+      put_rows<BM, RM>(ps, tx + 16 * c, ty, col);
+    }
+#pragma unroll
+    for (int r = 0; r < RM / 2; ++r) {
+      const u64 f = pk(corr[2 * r], corr[2 * r + 1]);
+#pragma unroll
+      for (int c = 0; c < DP / 16; ++c) o[r][c] = mul2(o[r][c], f);
     }
     __syncthreads();
-    product_nn<DP, RM, BN>(o, ps, kv, ty, tx);
+    product_nn<DP, RM, BN>(o, ps, vs, ty, tx);
   }
 #pragma unroll
   for (int r = 0; r < RM; ++r) {
     float sum = l[r];
 #pragma unroll
     for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    const int row = ty * RM + r;
+    const int row = ty + 16 * r;
     if (row >= t.rows) continue;
     const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // NaN stays NaN
     const int64_t tok = t.row0 + row;
@@ -197,7 +274,9 @@ __global__ void __launch_bounds__(kThreads) packed_simt_fwd_kernel(const PackedA
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int c = tx * 4 + g * 64 + i;
-        if (c < a.D) op[c] = from_acc<T>(o[r][g * 4 + i] * inv);
+        float x, y;
+        upk(o[r / 2][g * 4 + i], x, y);
+        if (c < a.D) op[c] = from_acc<T>((r % 2 ? y : x) * inv);
       }
   }
 }
@@ -208,7 +287,7 @@ __global__ void __launch_bounds__(kThreads) packed_simt_fwd_kernel(const PackedA
 template <int DP, int RM>
 struct BwdShape {
   static constexpr int BM = 16 * RM, BN = 16 * RM, CN = RM;
-  static constexpr int smem = (2 * (BM + BN) * (DP + 4) + 2 * BM * (BN + 4)) * 4 + 2 * BN * 4;
+  static constexpr int smem = (2 * (BM + BN) * (DP + 4) + 2 * BN * (BM + 4)) * 4 + 2 * BN * 4;
 };
 
 template <typename T, int VEC, int DP, int RM, bool DKV>
@@ -221,8 +300,8 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
   float* y1 = x2 + BM * LD;
   float* y2 = y1 + BN * LD;
   float* ps = y2 + BN * LD;            // P^T (DKV only)
-  float* ds = ps + BM * (BN + 4);      // dS or dS^T
-  float* cl = ds + BM * (BN + 4);      // log-sum-exp and delta of the columns (DKV)
+  float* ds = ps + BN * (BM + 4);      // dS or dS^T
+  float* cl = ds + BN * (BM + 4);      // log-sum-exp and delta of the columns (DKV)
   float* cd = cl + BN;
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   const int group = a.H / a.Hk;
@@ -243,13 +322,13 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
   const int head0 = DKV ? kvh * group : blockIdx.y, heads = DKV ? group : 1;
   const T* kp = (const T*)a.k + kvh * a.k_sh;
   const T* vp = (const T*)a.v + kvh * a.v_sh;
-  float acc1[RM][DP / 16], acc2[DKV ? RM : 1][DKV ? DP / 16 : 1];
+  u64 acc1[RM / 2][DP / 16], acc2[DKV ? RM / 2 : 1][DKV ? DP / 16 : 1];
 #pragma unroll
-  for (int r = 0; r < RM; ++r)
+  for (int r = 0; r < RM / 2; ++r)
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
-      acc1[r][c] = 0.f;
-      if (DKV) acc2[r][c] = 0.f;
+      acc1[r][c] = 0;
+      if (DKV) acc2[r][c] = 0;
     }
   float row_lse[RM], row_delta[RM];
   if (DKV) {
@@ -260,7 +339,7 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
     load_tile<T, VEC, DP>(x2, (const T*)a.go + t.row0 * a.go_st + head0 * a.go_sh, a.go_st, BM, t.rows, a.D);
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
-      const int row = ty * RM + r;
+      const int row = ty + 16 * r;
       const bool in = row < t.rows;
       row_lse[r] = in ? a.lse[(int64_t)head0 * a.Tq + t.row0 + row] * kLog2e : 0.f;
       row_delta[r] = in ? a.delta[(int64_t)head0 * a.Tq + t.row0 + row] : 0.f;
@@ -290,7 +369,7 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
       product_nt<DP, RM, CN>(dp, x2, y2, ty, tx);
 #pragma unroll
       for (int r = 0; r < RM; ++r) {
-        const int row = ty * RM + r;
+        const int row = ty + 16 * r;
         int64_t lo = 0, hi = row < t.rows ? valid : 0;  // columns that this row meets
         if (a.causal) {
           if (DKV) lo = first + row - shift - c0;       // queries from the key's place - shift on
@@ -301,10 +380,17 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
           const int col = tx + 16 * c;
           const float lse = DKV ? cl[col] : row_lse[r], delta = DKV ? cd[col] : row_delta[r];
           const bool in = col >= lo && col < hi;
-          const float p = in ? exp2f(fmaf(s[r][c], qscale, -lse)) : 0.f;
-          if (DKV) ps[row * (BN + 4) + col] = p;
-          ds[row * (BN + 4) + col] = in ? p * (dp[r][c] - delta) : 0.f;
+          s[r][c] = in ? exp2f(fmaf(s[r][c], qscale, -lse)) : 0.f;
+          dp[r][c] = in ? s[r][c] * (dp[r][c] - delta) : 0.f;
         }
+      }
+#pragma unroll
+      for (int c = 0; c < CN; ++c) {
+        float x[RM], y[RM];
+#pragma unroll
+        for (int r = 0; r < RM; ++r) x[r] = s[r][c], y[r] = dp[r][c];
+        if (DKV) put_rows<BM, RM>(ps, tx + 16 * c, ty, x);
+        put_rows<BM, RM>(ds, tx + 16 * c, ty, y);
       }
       __syncthreads();
       product_nn<DP, RM, BN>(acc1, ds, y1, ty, tx);
@@ -313,7 +399,7 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
   }
 #pragma unroll
   for (int r = 0; r < RM; ++r) {
-    const int row = ty * RM + r;
+    const int row = ty + 16 * r;
     if (row >= t.rows) continue;
     const int64_t at = DKV ? ((t.row0 + row) * a.Hk + kvh) * a.D : ((t.row0 + row) * a.H + head0) * a.D;
     T* d1 = (T*)(DKV ? a.dk : a.dq) + at;
@@ -324,8 +410,13 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
       for (int i = 0; i < 4; ++i) {
         const int c = tx * 4 + g * 64 + i;
         if (c < a.D) {
-          d1[c] = from_acc<T>(acc1[r][g * 4 + i] * a.scale);
-          if (DKV) d2[c] = from_acc<T>(acc2[r][g * 4 + i]);
+          float x, y;
+          upk(acc1[r / 2][g * 4 + i], x, y);
+          d1[c] = from_acc<T>((r % 2 ? y : x) * a.scale);
+          if constexpr (DKV) {
+            upk(acc2[r / 2][g * 4 + i], x, y);
+            d2[c] = from_acc<T>(r % 2 ? y : x);
+          }
         }
       }
   }
@@ -419,7 +510,7 @@ bool vec_ok(const PackedArgs& a, bool backward) {
 template <typename T, int VEC>
 int fwd_width(const PackedArgs& a, cudaStream_t st) {
   if (a.D <= 64) return fwd<T, VEC, 64, 8>(a, st);
-  if (a.D <= 128) return fwd<T, VEC, 128, 4>(a, st);
+  if (a.D <= 128) return fwd<T, VEC, 128, 8>(a, st);
   return fwd<T, VEC, 256, 4>(a, st);
 }
 template <typename T, int VEC>

@@ -12,14 +12,16 @@
 // tiles (dK, dV), one owns query tiles (dQ), so nothing is added by atomics and
 // every run gives the same bits, at 7 products in place of 5.
 //
-// 256 threads as 16 x 16; thread (ty, tx) holds rows ty + 16 r (r < RM) x columns
-// tx + 16 c (c < CN) of a score tile and the same rows x DP/16 columns of an output
-// tile.  All products are packed fp32 FMAs, which hold the FP32 pipe for two cycles
-// and leave every other issue slot to loads: scores pair neighbouring elements of
-// the summed dimension (both come as pairs out of 16-byte loads), outputs pair rows
-// (the probabilities are kept transposed, a thread's rows side by side).  Rows of
-// operand tiles have DP + 4 floats: the 16 lanes of a column load touch every bank
-// twice, a row load is a broadcast of two rows in different banks.
+// 256 threads as TY x TX; thread (ty, tx) holds rows ty + TY r (r < RM) x columns
+// tx + TX c (c < CN) of a score tile and the same rows x DP/TX columns of an output
+// tile.  Scores are packed fp32 FMAs over neighbouring elements of the summed dimension
+// (both operands come as pairs out of 16-byte loads): they hold the FP32 pipe for two
+// cycles and leave every other issue slot to loads.  Outputs are single FMAs: pairs would
+// need one operand doubled in registers, and the moves cost more than they save.  The
+// probabilities are kept transposed, a thread's rows side by side.  A warp is
+// 4 rows x 8 columns, so that both kinds of operand load are one shared-memory
+// wavefront (rows of DP + 4 floats: neighbouring rows lie in different banks): 12
+// wavefronts per 64 FMAs with 4 x 8 results per thread, 8 per 32 with 4 x 4.
 #include "attention_common.cuh"
 
 namespace tpo {
@@ -52,8 +54,8 @@ __device__ __forceinline__ void load_tile(float* dst, const T* src, int64_t stri
   }
 }
 
-// s[r][c] = sum_d a[ty + 16r][d] * b[tx + 16c][d]
-template <int DP, int RM, int CN>
+// s[r][c] = sum_d a[ty + TY r][d] * b[tx + TX c][d]
+template <int DP, int TY, int TX, int RM, int CN>
 __device__ __forceinline__ void product_nt(float (&s)[RM][CN], const float* a, const float* b, int ty,
                                            int tx) {
   constexpr int LD = DP + 4;
@@ -68,10 +70,10 @@ __device__ __forceinline__ void product_nt(float (&s)[RM][CN], const float* a, c
   for (int d = 0; d < DP; d += 4) {
     ulonglong2 bv[CN];
 #pragma unroll
-    for (int c = 0; c < CN; ++c) bv[c] = *reinterpret_cast<const ulonglong2*>(br + c * 16 * LD + d);
+    for (int c = 0; c < CN; ++c) bv[c] = *reinterpret_cast<const ulonglong2*>(br + c * TX * LD + d);
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
-      const ulonglong2 av = *reinterpret_cast<const ulonglong2*>(ar + r * 16 * LD + d);
+      const ulonglong2 av = *reinterpret_cast<const ulonglong2*>(ar + r * TY * LD + d);
 #pragma unroll
       for (int c = 0; c < CN; ++c) {
         acc[r][c] = fma2(av.x, bv[c].x, acc[r][c]);
@@ -102,34 +104,39 @@ __device__ __forceinline__ void put_rows(float* p, int j, int ty, const float (&
   }
 }
 
-// o[rp][4g + i] += sum_j (p[j][ty*RM + 2rp], p[j][ty*RM + 2rp + 1]) * v[j][tx*4 + 64g + i]
-template <int DP, int RM, int BN>
-__device__ __forceinline__ void product_nn(u64 (&o)[RM / 2][DP / 16], const float* p, const float* v,
+// o[r][4g + i] += sum_j p[j][ty*RM + r] * v[j][tx*4 + 4 TX g + i]
+template <int DP, int TY, int TX, int RM, int BN>
+__device__ __forceinline__ void product_nn(float (&o)[RM][DP / TX], const float* p, const float* v,
                                            int ty, int tx) {
-  constexpr int LDP = 16 * RM + 4;
+  constexpr int LDP = TY * RM + 4;
   const float* pr = p + ty * RM;
   const float* vr = v + tx * 4;
 #pragma unroll 4
   for (int j = 0; j < BN; ++j) {
-    u64 pv[RM / 2];
+    float pv[RM];
     if constexpr (RM % 4 == 0) {
 #pragma unroll
-      for (int r = 0; r < RM / 4; ++r) {
-        const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(pr + j * LDP + 4 * r);
-        pv[2 * r] = t.x, pv[2 * r + 1] = t.y;
+      for (int r = 0; r < RM; r += 4) {
+        const float4 t = *reinterpret_cast<const float4*>(pr + j * LDP + r);
+        pv[r] = t.x, pv[r + 1] = t.y, pv[r + 2] = t.z, pv[r + 3] = t.w;
       }
     } else {
 #pragma unroll
-      for (int r = 0; r < RM / 2; ++r) pv[r] = *reinterpret_cast<const u64*>(pr + j * LDP + 2 * r);
+      for (int r = 0; r < RM; r += 2) {
+        const float2 t = *reinterpret_cast<const float2*>(pr + j * LDP + r);
+        pv[r] = t.x, pv[r + 1] = t.y;
+      }
     }
 #pragma unroll
-    for (int g = 0; g < DP / 64; ++g) {
-      const float4 t = *reinterpret_cast<const float4*>(vr + j * (DP + 4) + g * 64);
-      const u64 vv[4] = {pk(t.x, t.x), pk(t.y, t.y), pk(t.z, t.z), pk(t.w, t.w)};
+    for (int g = 0; g < DP / TX / 4; ++g) {
+      const float4 t = *reinterpret_cast<const float4*>(vr + j * (DP + 4) + g * 4 * TX);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int r = 0; r < RM / 2; ++r) o[r][g * 4 + i] = fma2(pv[r], vv[i], o[r][g * 4 + i]);
+      for (int r = 0; r < RM; ++r) {
+        o[r][g * 4 + 0] = fmaf(pv[r], t.x, o[r][g * 4 + 0]);
+        o[r][g * 4 + 1] = fmaf(pv[r], t.y, o[r][g * 4 + 1]);
+        o[r][g * 4 + 2] = fmaf(pv[r], t.z, o[r][g * 4 + 2]);
+        o[r][g * 4 + 3] = fmaf(pv[r], t.w, o[r][g * 4 + 3]);
+      }
     }
   }
 }
@@ -170,20 +177,20 @@ struct InFlight {
 
 template <int DP, int RM>
 struct FwdShape {
-  static constexpr int BM = 16 * RM, BN = 64;
+  static constexpr int TY = 32, TX = 8, BM = TY * RM, BN = 64, CN = BN / TX;
   static constexpr int smem = ((BM + 2 * BN) * (DP + 4) + BN * (BM + 4)) * 4;
 };
 
 template <typename T, int VEC, int DP, int RM>
 __global__ void __launch_bounds__(kThreads) packed_simt_fwd_kernel(const PackedArgs a) {
   using Sh = FwdShape<DP, RM>;
-  constexpr int BM = Sh::BM, BN = Sh::BN, CN = 4;
+  constexpr int TY = Sh::TY, TX = Sh::TX, BM = Sh::BM, BN = Sh::BN, CN = Sh::CN;
   extern __shared__ float4 smem4[];
   float* qs = reinterpret_cast<float*>(smem4);
   float* ks = qs + BM * (DP + 4);
   float* vs = ks + BN * (DP + 4);
   float* ps = vs + BN * (DP + 4);
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
   const int head = blockIdx.y, kvh = head / (a.H / a.Hk);
   // causal rows late in a cloud see most keys: those blocks start first
   const int64_t slot = a.causal ? (int64_t)gridDim.x - 1 - blockIdx.x : blockIdx.x;
@@ -200,14 +207,14 @@ __global__ void __launch_bounds__(kThreads) packed_simt_fwd_kernel(const PackedA
   InFlight<T, VEC, DP, BN> next;
   if (nk > 0) next.get(kp, a.k_st, nk, a.D);
   load_tile<T, VEC, DP>(qs, (const T*)a.q + t.row0 * a.q_st + head * a.q_sh, a.q_st, BM, t.rows, a.D);
-  u64 o[RM / 2][DP / 16];
+  float o[RM][DP / TX];
   float m[RM], l[RM];
 #pragma unroll
   for (int r = 0; r < RM; ++r) {
     m[r] = -INFINITY;
     l[r] = 0.f;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) o[r / 2][c] = 0;
+    for (int c = 0; c < DP / TX; ++c) o[r][c] = 0.f;
   }
   for (int64_t j0 = 0; j0 < nk; j0 += BN) {
     const int valid = (int)min64(nk - j0, BN);
@@ -215,22 +222,22 @@ __global__ void __launch_bounds__(kThreads) packed_simt_fwd_kernel(const PackedA
     next.get(vp + j0 * a.v_st, a.v_st, nk - j0, a.D);
     __syncthreads();
     float s[RM][CN];
-    product_nt<DP, RM, CN>(s, qs, ks, ty, tx);
+    product_nt<DP, TY, TX, RM, CN>(s, qs, ks, ty, tx);
     next.put(vs);  // the last P V is over: every thread has passed the barrier above since
     if (j0 + BN < nk) next.get(kp + (j0 + BN) * a.k_st, a.k_st, nk - j0 - BN, a.D);
     float corr[RM];
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
       int64_t lim = valid;
-      if (a.causal) lim = min64(lim, first + ty + 16 * r + shift + 1 - j0);
+      if (a.causal) lim = min64(lim, first + ty + TY * r + shift + 1 - j0);
       float mx = m[r];
 #pragma unroll
       for (int c = 0; c < CN; ++c) {
-        s[r][c] = tx + 16 * c < lim ? s[r][c] * qscale : -INFINITY;
+        s[r][c] = tx + TX * c < lim ? s[r][c] * qscale : -INFINITY;
         mx = fmaxf(mx, s[r][c]);
       }
 #pragma unroll
-      for (int x = 8; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      for (int x = TX / 2; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
       const float base = mx == -INFINITY ? 0.f : mx;  // a row that has seen nothing yet
       corr[r] = exp2f(m[r] - base);
       float sum = 0.f;
@@ -247,36 +254,32 @@ __global__ void __launch_bounds__(kThreads) packed_simt_fwd_kernel(const PackedA
       float col[RM];
 #pragma unroll
       for (int r = 0; r < RM; ++r) col[r] = s[r][c];
-      put_rows<BM, RM>(ps, tx + 16 * c, ty, col);
+      put_rows<BM, RM>(ps, tx + TX * c, ty, col);
     }
 #pragma unroll
-    for (int r = 0; r < RM / 2; ++r) {
-      const u64 f = pk(corr[2 * r], corr[2 * r + 1]);
+    for (int r = 0; r < RM; ++r)
 #pragma unroll
-      for (int c = 0; c < DP / 16; ++c) o[r][c] = mul2(o[r][c], f);
-    }
+      for (int c = 0; c < DP / TX; ++c) o[r][c] *= corr[r];
     __syncthreads();
-    product_nn<DP, RM, BN>(o, ps, vs, ty, tx);
+    product_nn<DP, TY, TX, RM, BN>(o, ps, vs, ty, tx);
   }
 #pragma unroll
   for (int r = 0; r < RM; ++r) {
     float sum = l[r];
 #pragma unroll
-    for (int x = 8; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-    const int row = ty + 16 * r;
+    for (int x = TX / 2; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    const int row = ty + TY * r;
     if (row >= t.rows) continue;
     const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;  // NaN stays NaN
     const int64_t tok = t.row0 + row;
     if (tx == 0 && a.lse) a.lse[(int64_t)head * a.Tq + tok] = sum == 0.f ? -INFINITY : (m[r] + log2f(sum)) * kLn2;
     T* op = (T*)a.o + (tok * a.H + head) * a.D;
 #pragma unroll
-    for (int g = 0; g < DP / 64; ++g)
+    for (int g = 0; g < DP / TX / 4; ++g)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int c = tx * 4 + g * 64 + i;
-        float x, y;
-        upk(o[r / 2][g * 4 + i], x, y);
-        if (c < a.D) op[c] = from_acc<T>((r % 2 ? y : x) * inv);
+        const int c = tx * 4 + g * 4 * TX + i;
+        if (c < a.D) op[c] = from_acc<T>(o[r][g * 4 + i] * inv);
       }
   }
 }
@@ -286,14 +289,14 @@ __global__ void __launch_bounds__(kThreads) packed_simt_fwd_kernel(const PackedA
 // columns keys.  In both, s = X1 Y1^T and dp = X2 Y2^T.
 template <int DP, int RM>
 struct BwdShape {
-  static constexpr int BM = 16 * RM, BN = 16 * RM, CN = RM;
+  static constexpr int TY = 16, TX = 16, BM = TY * RM, BN = TX * RM, CN = RM;
   static constexpr int smem = (2 * (BM + BN) * (DP + 4) + 2 * BN * (BM + 4)) * 4 + 2 * BN * 4;
 };
 
 template <typename T, int VEC, int DP, int RM, bool DKV>
 __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedArgs a) {
   using Sh = BwdShape<DP, RM>;
-  constexpr int BM = Sh::BM, BN = Sh::BN, CN = Sh::CN, LD = DP + 4;
+  constexpr int TY = Sh::TY, TX = Sh::TX, BM = Sh::BM, BN = Sh::BN, CN = Sh::CN, LD = DP + 4;
   extern __shared__ float4 smem4[];
   float* x1 = reinterpret_cast<float*>(smem4);
   float* x2 = x1 + BM * LD;
@@ -303,7 +306,8 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
   float* ds = ps + BN * (BM + 4);      // dS or dS^T
   float* cl = ds + BN * (BM + 4);      // log-sum-exp and delta of the columns (DKV)
   float* cd = cl + BN;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int tx = lane % 8 + 8 * (warp % 2), ty = lane / 8 + 4 * (warp / 2);
   const int group = a.H / a.Hk;
   const int64_t slot = !DKV && a.causal ? (int64_t)gridDim.x - 1 - blockIdx.x : blockIdx.x;
   const Tile t = DKV ? find_tile(a.off_k, a.Tk, a.off_q, a.Tq, a.B, BM, slot)
@@ -322,13 +326,13 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
   const int head0 = DKV ? kvh * group : blockIdx.y, heads = DKV ? group : 1;
   const T* kp = (const T*)a.k + kvh * a.k_sh;
   const T* vp = (const T*)a.v + kvh * a.v_sh;
-  u64 acc1[RM / 2][DP / 16], acc2[DKV ? RM / 2 : 1][DKV ? DP / 16 : 1];
+  float acc1[RM][DP / TX], acc2[DKV ? RM : 1][DKV ? DP / TX : 1];
 #pragma unroll
-  for (int r = 0; r < RM / 2; ++r)
+  for (int r = 0; r < RM; ++r)
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c) {
-      acc1[r][c] = 0;
-      if (DKV) acc2[r][c] = 0;
+    for (int c = 0; c < DP / TX; ++c) {
+      acc1[r][c] = 0.f;
+      if (DKV) acc2[r][c] = 0.f;
     }
   float row_lse[RM], row_delta[RM];
   if (DKV) {
@@ -339,7 +343,7 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
     load_tile<T, VEC, DP>(x2, (const T*)a.go + t.row0 * a.go_st + head0 * a.go_sh, a.go_st, BM, t.rows, a.D);
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
-      const int row = ty + 16 * r;
+      const int row = ty + TY * r;
       const bool in = row < t.rows;
       row_lse[r] = in ? a.lse[(int64_t)head0 * a.Tq + t.row0 + row] * kLog2e : 0.f;
       row_delta[r] = in ? a.delta[(int64_t)head0 * a.Tq + t.row0 + row] : 0.f;
@@ -365,11 +369,11 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
       }
       __syncthreads();
       float s[RM][CN], dp[RM][CN];
-      product_nt<DP, RM, CN>(s, x1, y1, ty, tx);
-      product_nt<DP, RM, CN>(dp, x2, y2, ty, tx);
+      product_nt<DP, TY, TX, RM, CN>(s, x1, y1, ty, tx);
+      product_nt<DP, TY, TX, RM, CN>(dp, x2, y2, ty, tx);
 #pragma unroll
       for (int r = 0; r < RM; ++r) {
-        const int row = ty + 16 * r;
+        const int row = ty + TY * r;
         int64_t lo = 0, hi = row < t.rows ? valid : 0;  // columns that this row meets
         if (a.causal) {
           if (DKV) lo = first + row - shift - c0;       // queries from the key's place - shift on
@@ -377,7 +381,7 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
         }
 #pragma unroll
         for (int c = 0; c < CN; ++c) {
-          const int col = tx + 16 * c;
+          const int col = tx + TX * c;
           const float lse = DKV ? cl[col] : row_lse[r], delta = DKV ? cd[col] : row_delta[r];
           const bool in = col >= lo && col < hi;
           s[r][c] = in ? exp2f(fmaf(s[r][c], qscale, -lse)) : 0.f;
@@ -389,34 +393,29 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
         float x[RM], y[RM];
 #pragma unroll
         for (int r = 0; r < RM; ++r) x[r] = s[r][c], y[r] = dp[r][c];
-        if (DKV) put_rows<BM, RM>(ps, tx + 16 * c, ty, x);
-        put_rows<BM, RM>(ds, tx + 16 * c, ty, y);
+        if (DKV) put_rows<BM, RM>(ps, tx + TX * c, ty, x);
+        put_rows<BM, RM>(ds, tx + TX * c, ty, y);
       }
       __syncthreads();
-      product_nn<DP, RM, BN>(acc1, ds, y1, ty, tx);
-      if constexpr (DKV) product_nn<DP, RM, BN>(acc2, ps, y2, ty, tx);
+      product_nn<DP, TY, TX, RM, BN>(acc1, ds, y1, ty, tx);
+      if constexpr (DKV) product_nn<DP, TY, TX, RM, BN>(acc2, ps, y2, ty, tx);
     }
   }
 #pragma unroll
   for (int r = 0; r < RM; ++r) {
-    const int row = ty + 16 * r;
+    const int row = ty + TY * r;
     if (row >= t.rows) continue;
     const int64_t at = DKV ? ((t.row0 + row) * a.Hk + kvh) * a.D : ((t.row0 + row) * a.H + head0) * a.D;
     T* d1 = (T*)(DKV ? a.dk : a.dq) + at;
     T* d2 = DKV ? (T*)a.dv + at : nullptr;
 #pragma unroll
-    for (int g = 0; g < DP / 64; ++g)
+    for (int g = 0; g < DP / TX / 4; ++g)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int c = tx * 4 + g * 64 + i;
+        const int c = tx * 4 + g * 4 * TX + i;
         if (c < a.D) {
-          float x, y;
-          upk(acc1[r / 2][g * 4 + i], x, y);
-          d1[c] = from_acc<T>((r % 2 ? y : x) * a.scale);
-          if constexpr (DKV) {
-            upk(acc2[r / 2][g * 4 + i], x, y);
-            d2[c] = from_acc<T>(r % 2 ? y : x);
-          }
+          d1[c] = from_acc<T>(acc1[r][g * 4 + i] * a.scale);
+          if (DKV) d2[c] = from_acc<T>(acc2[r][g * 4 + i]);
         }
       }
   }
@@ -509,9 +508,9 @@ bool vec_ok(const PackedArgs& a, bool backward) {
 
 template <typename T, int VEC>
 int fwd_width(const PackedArgs& a, cudaStream_t st) {
-  if (a.D <= 64) return fwd<T, VEC, 64, 8>(a, st);
-  if (a.D <= 128) return fwd<T, VEC, 128, 8>(a, st);
-  return fwd<T, VEC, 256, 4>(a, st);
+  if (a.D <= 64) return fwd<T, VEC, 64, 4>(a, st);
+  if (a.D <= 128) return fwd<T, VEC, 128, 4>(a, st);
+  return fwd<T, VEC, 256, 2>(a, st);
 }
 template <typename T, int VEC>
 int bwd_width(const PackedArgs& a, cudaStream_t st) {

@@ -22,7 +22,7 @@ struct PackedArgs {
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, go_st, go_sh;  // token and head strides
   const int64_t *off_q, *off_k;
   void *o, *dq, *dk, *dv;
-  float *lse, *delta;
+  float *lse, *delta, *lse2;  // lse2: lse in base 2 (backward on the tensor cores), or null
   float* go_max;  // (H, Tq): largest |go| of each row (fp16 on the tensor cores), or null
   int64_t Tq, Tk;
   int B, H, Hk, D, causal;

@@ -49,6 +49,9 @@ struct FwdSmem {
 // 8 warps with a row per thread, 2 copy warps, 1 warp that issues products, and one
 // idle (registers are handed out per four warps anyway)
 constexpr int kThreads = 32 * 12, kCopyWarp = 8, kMmaWarp = 10;
+// 384 threads are launched with 168 registers each; the row warps draw what the others give
+constexpr int kRowRegs = 200, kOtherRegs = 104;
+static_assert(256 * kRowRegs + 128 * kOtherRegs <= kThreads * 168, "register split");
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1) packed_mma_fwd_kernel(const PackedArgs a) {
@@ -106,6 +109,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_fwd_kernel(const Packe
   // columns: S0 | S1 | O0 | O1; P over the first half of its S
   const uint32_t t_s = tmem, t_o = tmem + 256;
 
+  if (warp >= kCopyWarp) {
+  give_registers<kOtherRegs>();
   if (warp == kCopyWarp || warp == kCopyWarp + 1) {
     // ---- copies: Q, then K0 V0 K1 V1 ... through the ring ----
     const int tid = threadIdx.x - 32 * kCopyWarp;
@@ -194,8 +199,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_fwd_kernel(const Packe
       }
     }
     __syncwarp();
-  } else if (warp < kCopyWarp) {
+  }
+  } else {
     // ---- softmax: a thread owns a row ----
+    draw_registers<kRowRegs>();
     const int w = warp / 4, row = threadIdx.x % kTile;
     const uint32_t lane = (uint32_t)(warp % 4) * 32 << 16;
     const uint32_t ts = t_s + w * kTile + lane, to = t_o + w * DP + lane;
@@ -204,69 +211,78 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_fwd_kernel(const Packe
     // this row sees keys below `sees`
     const int64_t sees = a.causal ? min64(t.nb, first + w * kTile + row + shift + 1) : t.nb;
     float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < steps[w]; ++j) {
-      bar_wait(b_s + 8 * w, j & 1, abort, err);
-      tc_fence_after();
-      const int64_t left = sees - (int64_t)j * kTile;
-      const int lim = left >= kTile ? kTile : left > 0 ? (int)left : 0;
-      const bool whole = __all_sync(0xffffffffu, lim == kTile);
-      float mx = m;
+    // one step's row: masked columns count as -inf
+    auto step = [&](int j, int lim, auto masked) {
+      constexpr bool MASK = decltype(masked)::value;
+      uint32_t v[4][32];
 #pragma unroll
-      for (int c = 0; c < kTile; c += 32) {
-        uint32_t v[32];
-        tmem_ld32(ts + c, v);
-        tmem_wait_ld();
-        if (whole) {
+      for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, v[c]);
+      tmem_wait_ld();
+      if (MASK) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(v[i]));
-        } else {
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, c + i < lim ? __uint_as_float(v[i]) : -INFINITY);
-        }
+          for (int i = 0; i < 32; ++i) v[c][i] = c * 32 + i < lim ? v[c][i] : 0xff800000u;
       }
+      float mx[4];  // four chains: a maximum waits for the one before it
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        mx[c] = m;
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) mx[c] = max3(mx[c], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
+      }
+      const float top = max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
       // The base of the exponentials moves only when a maximum outgrows it by
       // more than 2^8: P stays below 256 (exact scaling by a power of the base is
       // undone by the division), and O is seldom rescaled.
-      const bool grow = (mx - m) * qscale > 8.f;  // also the first finite maximum: m = -inf
+      const bool grow = (top - m) * qscale > 8.f;  // also the first finite maximum: m = -inf
       if (__any_sync(0xffffffffu, grow)) {
-        const float corr = grow ? ex2((m - mx) * qscale) : 1.f;
-        if (grow) m = mx;
+        const float corr = grow ? ex2((m - top) * qscale) : 1.f;
+        if (grow) m = top;
         l *= corr;
         if (j > 0) {
-#pragma unroll
-          for (int c = 0; c < DP; c += 32) {
-            uint32_t v[32];
-            tmem_ld32(to + c, v);
+#pragma unroll 1
+          for (int c = 0; c < DP; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(to + c, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * corr);
-            tmem_st32(to + c, v);
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+            tmem_st16(to + c, o);
           }
         }
       }
       const float mb = m == -INFINITY ? 0.f : m * qscale;
-      float sum = 0.f;
+      const u64 q2 = pk(qscale, qscale), m2 = pk(-mb, -mb);
+      u64 sum[2] = {0, 0};
 #pragma unroll
-      for (int c = 0; c < kTile; c += 32) {
-        uint32_t v[32], p[16];
-        tmem_ld32(ts + c, v);
-        tmem_wait_ld();
+      for (int c = 0; c < 4; ++c) {
+        uint32_t p[16];
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float x = ex2(fmaf(__uint_as_float(v[i]), qscale, -mb)), y = ex2(fmaf(__uint_as_float(v[i + 1]), qscale, -mb));
-          if (!whole) {
-            x = c + i < lim ? x : 0.f;
-            y = c + i + 1 < lim ? y : 0.f;
-          }
-          sum += x + y;
-          p[i / 2] = pack2<T>(x, y);
+        for (int i = 0; i < 16; ++i) {
+          float x, y;
+          upk(fma2(pku(v[c][2 * i], v[c][2 * i + 1]), q2, m2), x, y);
+          x = ex2(x), y = ex2(y);
+          sum[i & 1] = add2(sum[i & 1], pk(x, y));
+          p[i] = pack2<T>(x, y);
         }
-        tmem_st16(ts + c / 2, p);
+        tmem_st16(ts + c * 16, p);
       }
-      l += sum;
+      float x, y;
+      upk(add2(sum[0], sum[1]), x, y);
+      l += x + y;
       tmem_wait_st();
       tc_fence_before();
       bar_arrive(b_p + 8 * w);
+    };
+    for (int j = 0; j < steps[w]; ++j) {
+      const int64_t left = sees - (int64_t)j * kTile;
+      const int lim = left >= kTile ? kTile : left > 0 ? (int)left : 0;
+      const bool whole = __all_sync(0xffffffffu, lim == kTile);
+      bar_wait(b_s + 8 * w, j & 1, abort, err);
+      tc_fence_after();
+      if (whole) step(j, lim, std::false_type{});
+      else step(j, lim, std::true_type{});
     }
     if (live && a.lse) a.lse[(int64_t)head * a.Tq + t.row0 + w * kTile + row] =
         l == 0.f ? -INFINITY : (m * qscale + log2f(l)) * kLn2;
@@ -325,7 +341,7 @@ template <int DP>
 struct BwdSmem {
   static constexpr int tile = kTile * DP * 2;
   static constexpr int stages = DP == 128 ? 4 : 8;
-  static constexpr int stats = 2 * tile + stages * tile;  // 128 floats per stage: lse with y1, delta with y2 (DKV)
+  static constexpr int stats = 2 * tile + stages * tile;  // 128 floats per stage: base-2 lse with y1, delta with y2 (DKV)
   static constexpr int bars = stats + stages * kTile * 4;
   static constexpr int total = bars + 256 + 1024;
 };
@@ -394,6 +410,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_bwd_kernel(const Packe
   // half become 32 at the half's start, so neither half overwrites the other's input.
   const uint32_t t_s = tmem, t_dp = tmem + 128, t_1 = tmem + 256, t_2 = tmem + 384;
 
+  if (warp >= kCopyWarp) {
+  give_registers<kOtherRegs>();
   if (warp == kCopyWarp || warp == kCopyWarp + 1) {
     const int tid = threadIdx.x - 32 * kCopyWarp;
     const T* kp = (const T*)a.k + kvh * a.k_sh;
@@ -430,12 +448,12 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_bwd_kernel(const Packe
           const int head = head0 + h;
           if (i & 1) copy_tile<T, DP>(dst, (const T*)a.go + tok * a.go_st + head * a.go_sh, a.go_st, t.nb - c0, a.D, tid);
           else copy_tile<T, DP>(dst, (const T*)a.q + tok * a.q_st + head * a.q_sh, a.q_st, t.nb - c0, a.D, tid);
-          const float* from = (i & 1 ? a.delta : a.lse) + (int64_t)head * a.Tq + tok;
+          const float* from = (i & 1 ? a.delta : a.lse2) + (int64_t)head * a.Tq + tok;
 #pragma unroll
           for (int r = tid; r < kTile; r += kCopyThreads) {
             const bool in = c0 + r < t.nb;
             asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(base + Sm::stats + (s * kTile + r) * 4),
-                         "l"(in ? from + r : a.lse), "r"(in ? 4 : 0)
+                         "l"(in ? from + r : a.lse2), "r"(in ? 4 : 0)
                          : "memory");
           }
         } else {
@@ -506,7 +524,9 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_bwd_kernel(const Packe
       mma_commit(b_done);
     }
     __syncwarp();
-  } else if (warp < kCopyWarp) {
+  }
+  } else {
+    draw_registers<kRowRegs>();
     const int half = warp / 4, row = threadIdx.x % kTile;
     const uint32_t lane = (uint32_t)(warp % 4) * 32 << 16;
     const uint32_t ts = t_s + half * 64 + lane, tdp = t_dp + half * 64 + lane;
@@ -528,9 +548,96 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_bwd_kernel(const Packe
     }
     float row_lse = 0.f, row_delta = 0.f;
     if (!DKV && live) {
-      row_lse = a.lse[(int64_t)head0 * a.Tq + t.row0 + row] * kLog2e;
+      row_lse = a.lse2[(int64_t)head0 * a.Tq + t.row0 + row];
       row_delta = a.delta[(int64_t)head0 * a.Tq + t.row0 + row];
     }
+    // one step's half row: P from S, then dS from dP
+    auto step_rows = [&](int j, int lo, int hi, auto masked) {
+      constexpr bool MASK = decltype(masked)::value;
+      const u64 q2 = pk(qscale, qscale);
+      u64 p[32];
+      {
+        const float* lse = stats + ((2 * j) % ST) * kTile + half * 64;  // base 2, negated below
+        uint32_t v[2][32];
+        bar_wait(b_s, j & 1, abort, err);
+        if (DKV) bar_wait(b_full + 8 * ((2 * j) % ST), (2 * j / ST) & 1, abort, err);
+        tc_fence_after();
+        tmem_ld32(ts, v[0]);
+        tmem_ld32(ts + 32, v[1]);
+        tmem_wait_ld();
+        if (!DKV) {  // S is read: the next product may overwrite it
+          tc_fence_before();
+          bar_arrive(b_p);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          u64 l0, l1;
+          if (DKV) {
+            const float4 f = *reinterpret_cast<const float4*>(lse + 2 * i);
+            l0 = pk(-f.x, -f.y), l1 = pk(-f.z, -f.w);
+          } else {
+            l0 = l1 = pk(-row_lse, -row_lse);
+          }
+          const uint32_t* s = &v[i / 16][(2 * i) % 32];
+          float x[4];
+          upk(fma2(pku(s[0], s[1]), q2, l0), x[0], x[1]);
+          upk(fma2(pku(s[2], s[3]), q2, l1), x[2], x[3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = ex2(x[e]);
+            if (MASK) x[e] = 2 * i + e >= lo && 2 * i + e < hi ? x[e] : 0.f;
+          }
+          p[i] = pk(x[0], x[1]), p[i + 1] = pk(x[2], x[3]);
+        }
+      }
+      if (DKV) {
+        uint32_t o[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          float x, y;
+          upk(p[i], x, y);
+          o[i] = pack2<T>(x, y);
+        }
+        tmem_st32(ts, o);
+        tmem_wait_st();
+        tc_fence_before();
+        bar_arrive(b_p);
+      }
+      const float* delta = stats + ((2 * j + 1) % ST) * kTile + half * 64;
+      bar_wait(b_dp, j & 1, abort, err);
+      if (DKV) bar_wait(b_full + 8 * ((2 * j + 1) % ST), ((2 * j + 1) / ST) & 1, abort, err);
+      tc_fence_after();
+      uint32_t v[2][32], o[32];
+      tmem_ld32(tdp, v[0]);
+      tmem_ld32(tdp + 32, v[1]);
+      tmem_wait_ld();
+#pragma unroll
+      for (int i = 0; i < 32; i += 2) {
+        u64 d0, d1;
+        if (DKV) {
+          const float4 f = *reinterpret_cast<const float4*>(delta + 2 * i);
+          d0 = pk(f.x, f.y), d1 = pk(f.z, f.w);
+        } else {
+          d0 = d1 = pk(row_delta, row_delta);
+        }
+        const uint32_t* s = &v[i / 16][(2 * i) % 32];
+        u64 a0 = mul2(p[i], sub2(pku(s[0], s[1]), d0)), a1 = mul2(p[i + 1], sub2(pku(s[2], s[3]), d1));
+        if (std::is_same<T, __half>::value) a0 = mul2(a0, pk(c, c)), a1 = mul2(a1, pk(c, c));
+        float x[4];
+        upk(a0, x[0], x[1]);
+        upk(a1, x[2], x[3]);
+        if (MASK) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = 2 * i + e >= lo && 2 * i + e < hi ? x[e] : 0.f;
+        }
+        o[i] = pack2<T>(x[0], x[1]);
+        o[i + 1] = pack2<T>(x[2], x[3]);
+      }
+      tmem_st32(tdp, o);
+      tmem_wait_st();
+      tc_fence_before();
+      bar_arrive(b_ds);
+    };
     int step = 0;
     for (int j = 0; j < n; ++j) {
       const int64_t c0 = c_begin + (int64_t)step * kTile + half * 64;
@@ -547,66 +654,8 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_bwd_kernel(const Packe
         hi = (int)min64(64, max64(0, end - c0));
       }
       const bool whole = __all_sync(0xffffffffu, lo == 0 && hi == 64);
-      const float* sl = stats + ((2 * j) % ST) * kTile + half * 64;
-      const float* sd = stats + ((2 * j + 1) % ST) * kTile + half * 64;
-      float p[64];
-      bar_wait(b_s, j & 1, abort, err);
-      if (DKV) bar_wait(b_full + 8 * ((2 * j) % ST), (2 * j / ST) & 1, abort, err);
-      tc_fence_after();
-#pragma unroll
-      for (int x = 0; x < 64; x += 32) {
-        uint32_t v[32], o[16];
-        tmem_ld32(ts + x, v);
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          float4 ls;
-          if (DKV) ls = *reinterpret_cast<const float4*>(sl + x + i);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float lse = DKV ? (e == 0 ? ls.x : e == 1 ? ls.y : e == 2 ? ls.z : ls.w) * kLog2e : row_lse;
-            float y = ex2(fmaf(__uint_as_float(v[i + e]), qscale, -lse));
-            if (!whole) y = x + i + e >= lo && x + i + e < hi ? y : 0.f;
-            p[x + i + e] = y;
-          }
-        }
-        if (DKV) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = pack2<T>(p[x + 2 * i], p[x + 2 * i + 1]);
-          tmem_st16(ts + x / 2, o);
-        }
-      }
-      if (DKV) tmem_wait_st();
-      tc_fence_before();
-      bar_arrive(b_p);
-      bar_wait(b_dp, j & 1, abort, err);
-      if (DKV) bar_wait(b_full + 8 * ((2 * j + 1) % ST), ((2 * j + 1) / ST) & 1, abort, err);
-      tc_fence_after();
-#pragma unroll
-      for (int x = 0; x < 64; x += 32) {
-        uint32_t v[32], o[16];
-        tmem_ld32(tdp + x, v);
-        tmem_wait_ld();
-#pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          float4 de;
-          if (DKV) de = *reinterpret_cast<const float4*>(sd + x + i);
-          float d[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float delta = DKV ? (e == 0 ? de.x : e == 1 ? de.y : e == 2 ? de.z : de.w) : row_delta;
-            d[e] = p[x + i + e] * (__uint_as_float(v[i + e]) - delta);
-            if (std::is_same<T, __half>::value) d[e] *= c;
-            if (!whole) d[e] = x + i + e >= lo && x + i + e < hi ? d[e] : 0.f;
-          }
-          o[i / 2] = pack2<T>(d[0], d[1]);
-          o[i / 2 + 1] = pack2<T>(d[2], d[3]);
-        }
-        tmem_st16(tdp + x / 2, o);
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      bar_arrive(b_ds);
+      if (whole) step_rows(j, lo, hi, std::false_type{});
+      else step_rows(j, lo, hi, std::true_type{});
     }
     if (n > 0) {
       bar_wait(b_done, 0, abort, err);

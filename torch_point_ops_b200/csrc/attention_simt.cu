@@ -421,8 +421,8 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
   }
 }
 
-// delta = dO . O per (head, token), and the row's largest |dO| where asked for; lpr
-// lanes per row, vectors of VEC.
+// delta = dO . O per (head, token), and where asked for the row's largest |dO| and its
+// log-sum-exp in base 2; lpr lanes per row, vectors of VEC.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) packed_delta_kernel(const PackedArgs a, int lpr) {
   const int64_t rows = a.Tq * a.H;
@@ -455,6 +455,7 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const PackedArgs a, i
     if (r < rows && l == 0) {
       a.delta[(int64_t)head * a.Tq + tok] = s;
       if (a.go_max) a.go_max[(int64_t)head * a.Tq + tok] = big;
+      if (a.lse2) a.lse2[(int64_t)head * a.Tq + tok] = a.lse[(int64_t)head * a.Tq + tok] * kLog2e;
     }
   }
 }

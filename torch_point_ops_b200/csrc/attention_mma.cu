@@ -1,11 +1,13 @@
 // Attention over packed clouds on the tensor cores: 16-bit inputs, width a
 // multiple of 8 up to 128, rows on 16-byte boundaries.
 //
-// Forward: a block owns 256 query rows of one (cloud, head) as two tiles of 128
-// and passes once over the keys in tiles of 128.  S = Q K^T and O += P V are
-// tcgen05 products with fp32 accumulators in tensor memory; P returns to tensor
-// memory as the A operand, over the columns of S that it was made from.  While
-// one tile's softmax runs, the tensor core works for the other tile.
+// All products are tcgen05 with fp32 accumulators in tensor memory (TMEM).  A block has
+// row warps (a thread owns a row of the score tile), two copy warps and one thread that
+// issues products; tiles travel through a ring in shared memory.
+//
+// Rounding to 16 bits happens to P before it multiplies V (and dO), and to dS before
+// it multiplies K and Q: the tensor cores take no wider operand beside 16-bit ones.
+// Every sum, maximum, P and dS themselves are fp32.
 #include <type_traits>
 
 #include "attention_common.cuh"
@@ -14,74 +16,141 @@
 namespace tpo {
 namespace {
 
-constexpr int kTile = 128;                        // rows of Q per softmax group, keys per step
-constexpr int kPanel = kTile * kPanelRow;         // 16 KB: 128 rows x 64 elements
-
-// 128 rows of a packed tensor into a swizzled tile, by the kCopyThreads threads of
-// the copy warps (t = index).  Rows at or beyond `valid` and columns at or beyond D
-// become zeros: nothing from another cloud enters a product (0 * NaN would).
+constexpr int kTile = 128;  // rows of a block's own tiles
 constexpr int kCopyThreads = 64;
-template <typename T, int DP>
+
+// ROWS rows of a packed tensor into a swizzled tile, by the copy warps (t = index).
+// Rows at or beyond `valid` and columns at or beyond D become zeros: nothing from
+// another cloud enters a product (0 * NaN would).
+template <typename T, int DP, int ROWS>
 __device__ __forceinline__ void copy_tile(uint32_t dst, const T* src, int64_t stride, int64_t valid, int D, int t) {
-  constexpr int CH = DP / 8;                 // 16-byte chunks per row
-  constexpr int STEP = kCopyThreads / CH;    // rows per pass
+  constexpr int CH = DP / 8;               // 16-byte chunks per row
+  constexpr int STEP = kCopyThreads / CH;  // rows per pass
   const int c = t % CH, r0 = t / CH;
-  const uint32_t at = dst + (c >> 3) * kPanel;
+  const uint32_t at = dst + (c >> 3) * ROWS * kPanelRow;
   const bool col = c * 8 < D;
   const T* p = src + (int64_t)r0 * stride + c * 8;
 #pragma unroll 8
-  for (int r = r0; r < kTile; r += STEP) {
+  for (int r = r0; r < ROWS; r += STEP) {
     const bool in = col && r < valid;
     cp_async16(at + r * kPanelRow + (((c & 7) ^ (r & 7)) << 4), in ? (const void*)p : (const void*)src, in);
     p += STEP * stride;
   }
 }
 
-// ---------------------------------------------------------------- forward
-template <int DP>
-struct FwdSmem {
-  static constexpr int q = kTile * DP * 2;          // one query tile
-  static constexpr int kv = kTile * DP * 2;         // one key or value tile
-  static constexpr int stages = DP == 128 ? 5 : 8;  // tiles in flight
-  static constexpr int bars = 2 * q + stages * kv;
-  static constexpr int total = bars + 256 + 1024;   // + alignment of the base
+// d (+)= x y^T over the width: x 128 rows, y NY rows, both K-major.
+template <typename T, int DP, int NY>
+__device__ __forceinline__ void mma_nt(uint32_t d, uint32_t x, uint32_t y) {
+  constexpr uint32_t id = mma_desc<T>(kTile, NY, false);
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks)
+    mma_ss(d, smem_desc(x + (ks / 4) * kTile * kPanelRow + (ks % 4) * 32, 16),
+           smem_desc(y + (ks / 4) * NY * kPanelRow + (ks % 4) * 32, 16), id, ks > 0);
+}
+// d (+)= p y over y's NY rows: p 128 rows of 16-bit values in TMEM, y MN-major.
+template <typename T, int DP, int NY>
+__device__ __forceinline__ void mma_nn(uint32_t d, uint32_t p, uint32_t y, bool more) {
+  constexpr uint32_t id = mma_desc<T>(kTile, DP, true);
+#pragma unroll
+  for (int ks = 0; ks < NY / 16; ++ks)
+    mma_ts(d, p + ks * 8, smem_desc(y + ks * 16 * kPanelRow, NY * kPanelRow), id, more || ks > 0);
+}
+
+// 32 accumulator columns times f as 16-bit values to global memory, whole chunks of 8.
+template <typename T>
+__device__ __forceinline__ void store32(T* out, const uint32_t (&v)[32], float f, int col, int D) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    if (col + i >= D) continue;
+    uint4 o;
+    uint32_t* ov = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      ov[e] = pack2<T>(__uint_as_float(v[i + 2 * e]) * f, __uint_as_float(v[i + 2 * e + 1]) * f);
+    *reinterpret_cast<uint4*>(out + col + i) = o;
+  }
+}
+
+// The ring of copied tiles.  A tile is announced by the copies themselves (each copy
+// thread's arrival follows its last copy); the reader orders them before the tensor
+// core's reads with a proxy fence.  A stage is handed back only where another tile will
+// fill it, so that no arrival is still on its way when the block ends.
+template <int ST>
+struct Ring {
+  uint32_t full, empty;  // barrier arrays
+  int tiles;
+  volatile int* abort;
+  __device__ __forceinline__ void wait_empty(int i) const {
+    if (i >= ST) bar_wait(empty + 8 * (i % ST), (i / ST - 1) & 1, abort, &g_attention_error);
+  }
+  __device__ __forceinline__ void announce(int i) const { cp_async_arrive(full + 8 * (i % ST)); }
+  __device__ __forceinline__ void wait_full(int i) const {
+    bar_wait(full + 8 * (i % ST), (i / ST) & 1, abort, &g_attention_error);
+  }
+  __device__ __forceinline__ void wait_operand(int i) const {
+    wait_full(i);
+    fence_async_smem();
+  }
+  __device__ __forceinline__ void release(int i) const {
+    if (i + ST < tiles) mma_commit(empty + 8 * (i % ST));
+  }
 };
-// 8 warps with a row per thread, 2 copy warps, 1 warp that issues products, and one
-// idle (registers are handed out per four warps anyway)
-constexpr int kThreads = 32 * 12, kCopyWarp = 8, kMmaWarp = 10;
-// 384 threads are launched with 168 registers each; the row warps draw what the others give
-constexpr int kRowRegs = 200, kOtherRegs = 104;
-static_assert(256 * kRowRegs + 128 * kOtherRegs <= kThreads * 168, "register split");
+
+// ---------------------------------------------------------------- forward
+// TILES tiles of 128 query rows pass once over the keys in tiles of 128.
+//
+// Width above 64: two query tiles per block (one block per SM), which share every key
+// and value tile; while one tile's softmax runs, the tensor core works for the
+// other.  TMEM is full (two S, two O), so P lies over the S that it was made from and
+// the next S waits for P V.
+//
+// Width up to 64: one tile per block and two blocks per SM, which hide each other's
+// start and end, and half the waste on short clouds; P has columns of its own, so the next
+// S is computed as soon as this one is read.
+template <int DP>
+struct Fwd {
+  static constexpr int TILES = DP == 128 ? 2 : 1;
+  static constexpr bool APART = DP == 64;  // P apart from S
+  static constexpr int threads = TILES * 128 + 128;
+  static constexpr int row_regs = 200, other_regs = TILES == 2 ? 104 : 56;
+  static constexpr int launch_regs = TILES == 2 ? 168 : 128;
+  static_assert(TILES * 128 * row_regs + 128 * other_regs <= threads * launch_regs, "register split");
+  static constexpr int tile = kTile * DP * 2;
+  static constexpr int stages = DP == 128 ? 5 : 5;
+  static constexpr int bars = (TILES + stages) * tile;
+  static constexpr int smem = bars + 256 + 1024;  // + alignment of the base
+  static constexpr int tmem = TILES * 256;
+  static constexpr int s = 0, p = APART ? 128 : 0, o = APART ? 192 : TILES * 128;  // columns
+};
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, 1) packed_mma_fwd_kernel(const PackedArgs a) {
-  using Sm = FwdSmem<DP>;
-  constexpr int ST = Sm::stages;
+__global__ void __launch_bounds__(Fwd<DP>::threads, Fwd<DP>::TILES == 2 ? 1 : 2)
+    packed_mma_fwd_kernel(const PackedArgs a) {
+  using F = Fwd<DP>;
+  constexpr int ST = F::stages, TILES = F::TILES;
+  constexpr int kCopyWarp = TILES * 4, kMmaWarp = kCopyWarp + 2;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_addr(smem_raw);
   const uint32_t base = (raw + 1023) & ~1023u;
-  const uint32_t sq = base, skv = base + 2 * Sm::q, bars = base + Sm::bars;
-  // barriers: queries full, stages full, stages empty, S full x 2, P full x 2, O done x 2
+  const uint32_t sq = base, skv = base + TILES * F::tile, bars = base + F::bars;
   const uint32_t b_q = bars, b_full = bars + 8, b_empty = b_full + 8 * ST, b_s = b_empty + 8 * ST, b_p = b_s + 16,
-                 b_o = b_p + 16, s_tmem = b_o + 16, s_abort = s_tmem + 4;
+                 b_o = b_p + 16, b_read = b_o + 16, s_tmem = b_read + 16, s_abort = s_tmem + 4;
   volatile int* abort = reinterpret_cast<volatile int*>(smem_raw + (s_abort - raw));
   unsigned* err = &g_attention_error;
 
   const int warp = threadIdx.x / 32, head = blockIdx.y, kvh = head / (a.H / a.Hk);
   const int64_t slot = a.causal ? (int64_t)gridDim.x - 1 - blockIdx.x : blockIdx.x;
-  const Tile t = find_tile(a.off_q, a.Tq, a.off_k, a.Tk, a.B, 2 * kTile, slot);
+  const Tile t = find_tile(a.off_q, a.Tq, a.off_k, a.Tk, a.B, TILES * kTile, slot);
   if (t.rows <= 0) return;
   const int64_t shift = t.nb - t.na, first = t.row0 - t.a0;
-  // keys that tile w meets, and its steps
-  int64_t nk[2];
-  int steps[2];
+  int steps[TILES], n = 0;  // key tiles that each query tile meets
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
+  for (int w = 0; w < TILES; ++w) {
     const int rows = max(0, min(kTile, t.rows - w * kTile));
-    nk[w] = rows == 0 ? 0 : a.causal ? min64(t.nb, max64(first + w * kTile + rows + shift, 0)) : t.nb;
-    steps[w] = (int)((nk[w] + kTile - 1) / kTile);
+    const int64_t nk = rows == 0 ? 0 : a.causal ? min64(t.nb, max64(first + w * kTile + rows + shift, 0)) : t.nb;
+    steps[w] = (int)((nk + kTile - 1) / kTile);
+    n = max(n, steps[w]);
   }
-  const int n = max(steps[0], steps[1]);
 
   if (warp == kMmaWarp) {
     if (threadIdx.x % 32 == 0) {
@@ -90,124 +159,95 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_fwd_kernel(const Packe
         bar_init(b_full + 8 * i, kCopyThreads);
         bar_init(b_empty + 8 * i, 1);
       }
-      for (int w = 0; w < 2; ++w) {
+      for (int w = 0; w < TILES; ++w) {
         bar_init(b_s + 8 * w, 1);
         bar_init(b_p + 8 * w, 128);
         bar_init(b_o + 8 * w, 1);
+        bar_init(b_read + 8 * w, 128);
       }
       *abort = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
-    tmem_alloc(s_tmem, 512);
+    tmem_alloc(s_tmem, F::tmem);
     tc_fence_before();
   }
   __syncthreads();
   tc_fence_after();
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(s_tmem));
-  // columns: S0 | S1 | O0 | O1; P over the first half of its S
-  const uint32_t t_s = tmem, t_o = tmem + 256;
+  const uint32_t t_s = tmem + F::s, t_p = tmem + F::p, t_o = tmem + F::o;
+  const Ring<ST> ring = {b_full, b_empty, 2 * n, abort};
 
   if (warp >= kCopyWarp) {
-  give_registers<kOtherRegs>();
-  if (warp == kCopyWarp || warp == kCopyWarp + 1) {
-    // ---- copies: Q, then K0 V0 K1 V1 ... through the ring ----
-    const int tid = threadIdx.x - 32 * kCopyWarp;
-    const T* qp = (const T*)a.q + t.row0 * a.q_st + head * a.q_sh;
-    const T* kp = (const T*)a.k + t.b0 * a.k_st + kvh * a.k_sh;
-    const T* vp = (const T*)a.v + t.b0 * a.v_st + kvh * a.v_sh;
-    if (n > 0) {
+    give_registers<F::other_regs>();
+    if (warp < kMmaWarp) {
+      // ---- copies: Q, then K0 V0 K1 V1 ... ----
+      const int tid = threadIdx.x - 32 * kCopyWarp;
+      if (n > 0) {
+        const T* qp = (const T*)a.q + t.row0 * a.q_st + head * a.q_sh;
 #pragma unroll
-      for (int w = 0; w < 2; ++w)
-        copy_tile<T, DP>(sq + w * Sm::q, qp + (int64_t)w * kTile * a.q_st, a.q_st, t.rows - w * kTile, a.D, tid);
-      cp_async_commit();
-      int told = -1;  // tiles below this one are announced; -1: Q is not yet
-      auto announce = [&](int upto) {  // all copies of tiles < upto have landed
-        fence_async_smem();
-        if (told < 0) bar_arrive(b_q), told = 0;
-        for (; told < upto; ++told) bar_arrive(b_full + 8 * (told % ST));
-      };
-      for (int i = 0; i < 2 * n; ++i) {
-        const int s = i % ST;
-        if (i >= ST) {
-          const uint32_t parity = (i / ST - 1) & 1;
-          if (!bar_try(b_empty + 8 * s, parity)) {
-            cp_async_wait<0>();
-            announce(i);
-            bar_wait(b_empty + 8 * s, parity, abort, err);
-          }
+        for (int w = 0; w < TILES; ++w)
+          copy_tile<T, DP, kTile>(sq + w * F::tile, qp + (int64_t)w * kTile * a.q_st, a.q_st, t.rows - w * kTile, a.D, tid);
+        cp_async_arrive(b_q);
+        const T* kp = (const T*)a.k + t.b0 * a.k_st + kvh * a.k_sh;
+        const T* vp = (const T*)a.v + t.b0 * a.v_st + kvh * a.v_sh;
+        for (int i = 0; i < 2 * n; ++i) {
+          ring.wait_empty(i);
+          const int64_t j = (int64_t)(i >> 1) * kTile;
+          const uint32_t dst = skv + (i % ST) * F::tile;
+          if (i & 1) copy_tile<T, DP, kTile>(dst, vp + j * a.v_st, a.v_st, t.nb - j, a.D, tid);
+          else copy_tile<T, DP, kTile>(dst, kp + j * a.k_st, a.k_st, t.nb - j, a.D, tid);
+          ring.announce(i);
         }
-        const int64_t j = (int64_t)(i >> 1) * kTile;
-        if (i & 1) copy_tile<T, DP>(skv + s * Sm::kv, vp + j * a.v_st, a.v_st, t.nb - j, a.D, tid);
-        else copy_tile<T, DP>(skv + s * Sm::kv, kp + j * a.k_st, a.k_st, t.nb - j, a.D, tid);
-        cp_async_commit();
-        cp_async_wait<1>();
-        announce(i);
+        cp_async_wait_all();
       }
-      cp_async_wait<0>();
-      announce(2 * n);
-    }
-  } else if (warp == kMmaWarp) {
-    // ---- products, issued by one thread ----
-    if (threadIdx.x % 32 == 0 && n > 0) {
-      constexpr uint32_t id_s = mma_desc<T>(kTile, kTile, false), id_o = mma_desc<T>(kTile, DP, true);
+    } else if (warp == kMmaWarp && threadIdx.x % 32 == 0 && n > 0) {
+      // ---- products ----
       auto score = [&](int w, int j) {  // S_w = Q_w K_j^T
-        const uint32_t k = skv + ((2 * j) % ST) * Sm::kv, q = sq + w * Sm::q;
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-          const uint32_t at = (ks / 4) * kPanel + (ks % 4) * 32;
-          mma_ss(t_s + w * kTile, smem_desc(q + at, 16), smem_desc(k + at, 16), id_s, ks > 0);
-        }
+        mma_nt<T, DP, kTile>(t_s + w * kTile, sq + w * F::tile, skv + ((2 * j) % ST) * F::tile);
+        mma_commit(b_s + 8 * w);
       };
-      auto wait_tile = [&](int i) { bar_wait(b_full + 8 * (i % ST), (i / ST) & 1, abort, err); };
       bar_wait(b_q, 0, abort, err);
-      wait_tile(0);
-      for (int w = 0; w < 2; ++w)
-        if (steps[w] > 0) {
-          score(w, 0);
-          mma_commit(b_s + 8 * w);
-        }
-      // a stage is handed back only where another tile will fill it, so that no
-      // arrival is still on its way when the block ends
-      auto release = [&](int i) {
-        if (i + ST < 2 * n) mma_commit(b_empty + 8 * (i % ST));
-      };
-      release(0);
+      ring.wait_operand(0);
+#pragma unroll
+      for (int w = 0; w < TILES; ++w)
+        if (steps[w] > 0) score(w, 0);
+      ring.release(0);
       for (int j = 0; j < n; ++j) {
         const int iv = 2 * j + 1, ik = 2 * j + 2;
-        wait_tile(iv);
-        if (j + 1 < n) wait_tile(ik);
-        const uint32_t v = skv + (iv % ST) * Sm::kv;
-        for (int w = 0; w < 2; ++w) {
+        const uint32_t v = skv + (iv % ST) * F::tile;
+        if (F::APART && j + 1 < n) {
+          bar_wait(b_read, j & 1, abort, err);
+          tc_fence_after();
+          ring.wait_operand(ik);
+          score(0, j + 1);
+          ring.release(ik);
+        }
+        ring.wait_operand(iv);
+        if (!F::APART && j + 1 < n) ring.wait_operand(ik);
+#pragma unroll
+        for (int w = 0; w < TILES; ++w) {
           if (j >= steps[w]) continue;
           bar_wait(b_p + 8 * w, j & 1, abort, err);
           tc_fence_after();
-#pragma unroll
-          for (int ks = 0; ks < kTile / 16; ++ks)
-            mma_ts(t_o + w * DP, t_s + w * kTile + ks * 8, smem_desc(v + ks * 16 * kPanelRow, kPanel), id_o,
-                   j > 0 || ks > 0);
-          if (j + 1 < steps[w]) {
-            score(w, j + 1);
-            mma_commit(b_s + 8 * w);
-          } else {
-            mma_commit(b_o + 8 * w);
-          }
+          mma_nn<T, DP, kTile>(t_o + w * DP, t_p + w * kTile, v, j > 0);
+          if (F::APART || j + 1 == steps[w]) mma_commit(b_o + 8 * w);
+          else score(w, j + 1);
         }
-        release(iv);
-        release(ik);
+        ring.release(iv);
+        if (!F::APART) ring.release(ik);
       }
     }
-    __syncwarp();
-  }
   } else {
     // ---- softmax: a thread owns a row ----
-    draw_registers<kRowRegs>();
+    draw_registers<F::row_regs>();
     const int w = warp / 4, row = threadIdx.x % kTile;
     const uint32_t lane = (uint32_t)(warp % 4) * 32 << 16;
-    const uint32_t ts = t_s + w * kTile + lane, to = t_o + w * DP + lane;
+    const uint32_t ts = t_s + w * kTile + lane, tp = t_p + w * kTile + lane, to = t_o + w * DP + lane;
     const bool live = w * kTile + row < t.rows;
     const float qscale = a.scale * kLog2e;
+    const int my_steps = w == 0 ? steps[0] : steps[TILES - 1];
     // this row sees keys below `sees`
     const int64_t sees = a.causal ? min64(t.nb, first + w * kTile + row + shift + 1) : t.nb;
     float m = -INFINITY, l = 0.f;
@@ -218,6 +258,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_fwd_kernel(const Packe
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, v[c]);
       tmem_wait_ld();
+      if (F::APART) {
+        tc_fence_before();
+        bar_arrive(b_read);
+      }
       if (MASK) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
@@ -232,6 +276,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_fwd_kernel(const Packe
         for (int i = 0; i < 32; i += 2) mx[c] = max3(mx[c], __uint_as_float(v[c][i]), __uint_as_float(v[c][i + 1]));
       }
       const float top = max3(mx[0], mx[1], fmaxf(mx[2], mx[3]));
+      if (F::APART && j > 0) {  // O and P are free: P V of the step before is done
+        bar_wait(b_o, (j - 1) & 1, abort, err);
+        tc_fence_after();
+      }
       // The base of the exponentials moves only when a maximum outgrows it by
       // more than 2^8: P stays below 256 (exact scaling by a power of the base is
       // undone by the division), and O is seldom rescaled.
@@ -266,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_fwd_kernel(const Packe
           sum[i & 1] = add2(sum[i & 1], pk(x, y));
           p[i] = pack2<T>(x, y);
         }
-        tmem_st16(ts + c * 16, p);
+        tmem_st16(tp + c * 16, p);
       }
       float x, y;
       upk(add2(sum[0], sum[1]), x, y);
@@ -275,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_fwd_kernel(const Packe
       tc_fence_before();
       bar_arrive(b_p + 8 * w);
     };
-    for (int j = 0; j < steps[w]; ++j) {
+    for (int j = 0; j < my_steps; ++j) {
       const int64_t left = sees - (int64_t)j * kTile;
       const int lim = left >= kTile ? kTile : left > 0 ? (int)left : 0;
       const bool whole = __all_sync(0xffffffffu, lim == kTile);
@@ -284,43 +332,32 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_fwd_kernel(const Packe
       if (whole) step(j, lim, std::false_type{});
       else step(j, lim, std::true_type{});
     }
-    if (live && a.lse) a.lse[(int64_t)head * a.Tq + t.row0 + w * kTile + row] =
-        l == 0.f ? -INFINITY : (m * qscale + log2f(l)) * kLn2;
+    const int64_t tok = t.row0 + w * kTile + row;
+    if (live && a.lse) a.lse[(int64_t)head * a.Tq + tok] = l == 0.f ? -INFINITY : (m * qscale + log2f(l)) * kLn2;
     const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
-    T* op = (T*)a.o + ((t.row0 + w * kTile + row) * a.H + head) * a.D;
-    if (steps[w] > 0) {
-      bar_wait(b_o + 8 * w, 0, abort, err);
+    T* op = (T*)a.o + (tok * a.H + head) * a.D;
+    if (my_steps > 0) {
+      bar_wait(b_o + 8 * w, F::APART ? (my_steps - 1) & 1 : 0, abort, err);
       tc_fence_after();
     }
 #pragma unroll
     for (int c = 0; c < DP; c += 32) {
       uint32_t v[32];
-      if (steps[w] > 0) {
+      if (my_steps > 0) {
         tmem_ld32(to + c, v);
         tmem_wait_ld();
       } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = 0;
       }
-      if (live) {
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          if (c + i >= a.D) continue;
-          uint4 o;
-          uint32_t* ov = reinterpret_cast<uint32_t*>(&o);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            ov[e] = pack2<T>(__uint_as_float(v[i + 2 * e]) * inv, __uint_as_float(v[i + 2 * e + 1]) * inv);
-          *reinterpret_cast<uint4*>(op + c + i) = o;
-        }
-      }
+      if (live) store32<T>(op, v, inv, c, a.D);
     }
     tc_fence_before();
   }
   __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after();
-    tmem_free(tmem, 512);
+    tmem_free(tmem, F::tmem);
   }
 }
 
@@ -330,20 +367,27 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_fwd_kernel(const Packe
 // streamed columns are queries (y1 = Q, y2 = dO) of every head of the group;
 // acc1 = dK += dS^T Q, acc2 = dV += P^T dO.  Otherwise rows are 128 queries
 // (x1 = Q, x2 = dO), columns keys (y1 = K, y2 = V), acc1 = dQ += dS K.  In both,
-// S = x1 y1^T, dP = x2 y2^T, and P and dS go back to tensor memory as A operands.
+// S = x1 y1^T, dP = x2 y2^T, and P and dS go back to TMEM as A operands, over S and dP.
 // Each sum has one owner: no atomics, the same bits in every run.
 //
-// Two phases alternate on single buffers: while the 256 threads turn S into P the
-// tensor core runs acc1 of the step before and dP; while they turn dP into dS it
-// runs acc2 and the next S.  A row's columns are shared by two threads (halves of
-// 64), so the fp32 P stay in registers from one phase to the other.
+// Columns come in tiles of 64.  Width above 64: two groups of row warps with their own S
+// and dP take tiles in turn, so the tensor core works for one while the other
+// computes.  Width up to 64: one group per block, two blocks per SM.
+constexpr int kCols = 64;
 template <int DP>
-struct BwdSmem {
-  static constexpr int tile = kTile * DP * 2;
-  static constexpr int stages = DP == 128 ? 4 : 8;
-  static constexpr int stats = 2 * tile + stages * tile;  // 128 floats per stage: base-2 lse with y1, delta with y2 (DKV)
-  static constexpr int bars = stats + stages * kTile * 4;
-  static constexpr int total = bars + 256 + 1024;
+struct Bwd {
+  static constexpr int GROUPS = DP == 128 ? 2 : 1;
+  static constexpr int threads = GROUPS * 128 + 128;
+  static constexpr int row_regs = 200, other_regs = GROUPS == 2 ? 104 : 56;
+  static constexpr int launch_regs = GROUPS == 2 ? 168 : 128;
+  static_assert(GROUPS * 128 * row_regs + 128 * other_regs <= threads * launch_regs, "register split");
+  static constexpr int own = kTile * DP * 2, tile = kCols * DP * 2;
+  static constexpr int stages = 8;
+  static constexpr int stats = 2 * own + stages * tile;  // 64 floats per stage: base-2 lse with y1, delta with y2 (DKV)
+  static constexpr int bars = stats + stages * kCols * 4;
+  static constexpr int smem = bars + 256 + 1024;
+  static constexpr int tmem = GROUPS * 256;
+  static constexpr int acc1 = GROUPS * 128, acc2 = acc1 + DP;  // columns; S and dP of group g at 128 g and 128 g + 64
 };
 
 // 2^-e for the power of two 2^e at or below the largest |dO| that a sum meets: brings
@@ -354,16 +398,18 @@ __device__ __forceinline__ float grad_scale(float largest) {
 }
 
 template <typename T, int DP, bool DKV>
-__global__ void __launch_bounds__(kThreads, 1) packed_mma_bwd_kernel(const PackedArgs a) {
-  using Sm = BwdSmem<DP>;
-  constexpr int ST = Sm::stages;
+__global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2)
+    packed_mma_bwd_kernel(const PackedArgs a) {
+  using W = Bwd<DP>;
+  constexpr int ST = W::stages, GROUPS = W::GROUPS;
+  constexpr int kCopyWarp = GROUPS * 4, kMmaWarp = kCopyWarp + 2;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_addr(smem_raw);
   const uint32_t base = (raw + 1023) & ~1023u;
-  const uint32_t sx = base, sy = base + 2 * Sm::tile, bars = base + Sm::bars;
-  const float* stats = reinterpret_cast<const float*>(smem_raw + (base + Sm::stats - raw));
-  const uint32_t b_x = bars, b_full = bars + 8, b_empty = b_full + 8 * ST, b_s = b_empty + 8 * ST, b_dp = b_s + 8,
-                 b_p = b_dp + 8, b_ds = b_p + 8, b_done = b_ds + 8, s_tmem = b_done + 8, s_abort = s_tmem + 4;
+  const uint32_t sx1 = base, sx2 = base + W::own, sy = base + 2 * W::own, bars = base + W::bars;
+  const float* stats = reinterpret_cast<const float*>(smem_raw + (base + W::stats - raw));
+  const uint32_t b_x = bars, b_full = bars + 8, b_empty = b_full + 8 * ST, b_s = b_empty + 8 * ST, b_dp = b_s + 16,
+                 b_p = b_dp + 16, b_ds = b_p + 16, b_done = b_ds + 16, s_tmem = b_done + 8, s_abort = s_tmem + 4;
   volatile int* abort = reinterpret_cast<volatile int*>(smem_raw + (s_abort - raw));
   unsigned* err = &g_attention_error;
 
@@ -375,10 +421,10 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_bwd_kernel(const Packe
   const int64_t nq = DKV ? t.nb : t.na, nkeys = DKV ? t.na : t.nb, shift = nkeys - nq, first = t.row0 - t.a0;
   int64_t c_begin = 0, c_end = t.nb;  // columns that any row of the tile meets
   if (a.causal) {
-    if (DKV) c_begin = max64(0, first - shift) / kTile * kTile;
+    if (DKV) c_begin = max64(0, first - shift) / kCols * kCols;
     else c_end = min64(c_end, max64(first + t.rows + shift, 0));
   }
-  const int per_head = (int)max64(0, (c_end - c_begin + kTile - 1) / kTile);
+  const int per_head = (int)max64(0, (c_end - c_begin + kCols - 1) / kCols);
   const int kvh = DKV ? blockIdx.y : blockIdx.y / group;
   const int head0 = DKV ? kvh * group : blockIdx.y;
   const int n = per_head * (DKV ? group : 1);
@@ -390,146 +436,106 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_bwd_kernel(const Packe
         bar_init(b_full + 8 * i, kCopyThreads);
         bar_init(b_empty + 8 * i, 1);
       }
-      bar_init(b_s, 1);
-      bar_init(b_dp, 1);
-      bar_init(b_p, 256);
-      bar_init(b_ds, 256);
+      for (int g = 0; g < GROUPS; ++g) {
+        bar_init(b_s + 8 * g, 1);
+        bar_init(b_dp + 8 * g, 1);
+        bar_init(b_p + 8 * g, 128);
+        bar_init(b_ds + 8 * g, 128);
+      }
       bar_init(b_done, 1);
       *abort = 0;
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
-    tmem_alloc(s_tmem, 512);
+    tmem_alloc(s_tmem, W::tmem);
     tc_fence_before();
   }
   __syncthreads();
   tc_fence_after();
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(s_tmem));
-  // columns: S | dP | acc1 | acc2.  P lies over S and dS over dP: the 64 columns of a
-  // half become 32 at the half's start, so neither half overwrites the other's input.
-  const uint32_t t_s = tmem, t_dp = tmem + 128, t_1 = tmem + 256, t_2 = tmem + 384;
+  const uint32_t t_1 = tmem + W::acc1, t_2 = tmem + W::acc2;
+  const Ring<ST> ring = {b_full, b_empty, 2 * n, abort};
 
   if (warp >= kCopyWarp) {
-  give_registers<kOtherRegs>();
-  if (warp == kCopyWarp || warp == kCopyWarp + 1) {
-    const int tid = threadIdx.x - 32 * kCopyWarp;
-    const T* kp = (const T*)a.k + kvh * a.k_sh;
-    const T* vp = (const T*)a.v + kvh * a.v_sh;
-    if (n > 0) {
-      if (DKV) {
-        copy_tile<T, DP>(sx, kp + t.row0 * a.k_st, a.k_st, t.rows, a.D, tid);
-        copy_tile<T, DP>(sx + Sm::tile, vp + t.row0 * a.v_st, a.v_st, t.rows, a.D, tid);
-      } else {
-        copy_tile<T, DP>(sx, (const T*)a.q + t.row0 * a.q_st + head0 * a.q_sh, a.q_st, t.rows, a.D, tid);
-        copy_tile<T, DP>(sx + Sm::tile, (const T*)a.go + t.row0 * a.go_st + head0 * a.go_sh, a.go_st, t.rows, a.D, tid);
-      }
-      cp_async_commit();
-      int told = -1;
-      auto announce = [&](int upto) {
-        fence_async_smem();
-        if (told < 0) bar_arrive(b_x), told = 0;
-        for (; told < upto; ++told) bar_arrive(b_full + 8 * (told % ST));
-      };
-      int h = 0, step = 0;
-      for (int i = 0; i < 2 * n; ++i) {
-        const int s = i % ST;
-        if (i >= ST) {
-          const uint32_t parity = (i / ST - 1) & 1;
-          if (!bar_try(b_empty + 8 * s, parity)) {
-            cp_async_wait<0>();
-            announce(i);
-            bar_wait(b_empty + 8 * s, parity, abort, err);
-          }
-        }
-        const int64_t c0 = c_begin + (int64_t)step * kTile, tok = t.b0 + c0;
-        const uint32_t dst = sy + s * Sm::tile;
+    give_registers<W::other_regs>();
+    if (warp < kMmaWarp) {
+      // ---- copies: x1 x2, then y1 y2 of column tile 0, 1, ... (DKV: head after head) ----
+      const int tid = threadIdx.x - 32 * kCopyWarp;
+      const T* kp = (const T*)a.k + kvh * a.k_sh;
+      const T* vp = (const T*)a.v + kvh * a.v_sh;
+      if (n > 0) {
         if (DKV) {
-          const int head = head0 + h;
-          if (i & 1) copy_tile<T, DP>(dst, (const T*)a.go + tok * a.go_st + head * a.go_sh, a.go_st, t.nb - c0, a.D, tid);
-          else copy_tile<T, DP>(dst, (const T*)a.q + tok * a.q_st + head * a.q_sh, a.q_st, t.nb - c0, a.D, tid);
-          const float* from = (i & 1 ? a.delta : a.lse2) + (int64_t)head * a.Tq + tok;
-#pragma unroll
-          for (int r = tid; r < kTile; r += kCopyThreads) {
-            const bool in = c0 + r < t.nb;
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(base + Sm::stats + (s * kTile + r) * 4),
-                         "l"(in ? from + r : a.lse2), "r"(in ? 4 : 0)
-                         : "memory");
-          }
+          copy_tile<T, DP, kTile>(sx1, kp + t.row0 * a.k_st, a.k_st, t.rows, a.D, tid);
+          copy_tile<T, DP, kTile>(sx2, vp + t.row0 * a.v_st, a.v_st, t.rows, a.D, tid);
         } else {
-          if (i & 1) copy_tile<T, DP>(dst, vp + tok * a.v_st, a.v_st, t.nb - c0, a.D, tid);
-          else copy_tile<T, DP>(dst, kp + tok * a.k_st, a.k_st, t.nb - c0, a.D, tid);
+          copy_tile<T, DP, kTile>(sx1, (const T*)a.q + t.row0 * a.q_st + head0 * a.q_sh, a.q_st, t.rows, a.D, tid);
+          copy_tile<T, DP, kTile>(sx2, (const T*)a.go + t.row0 * a.go_st + head0 * a.go_sh, a.go_st, t.rows, a.D, tid);
         }
-        if (i & 1) {
-          if (++step == per_head) step = 0, ++h;
+        cp_async_arrive(b_x);
+        int h = 0, step = 0;
+        for (int i = 0; i < 2 * n; ++i) {
+          ring.wait_empty(i);
+          const int s = i % ST;
+          const int64_t c0 = c_begin + (int64_t)step * kCols, tok = t.b0 + c0;
+          const uint32_t dst = sy + s * W::tile;
+          if (DKV) {
+            const int head = head0 + h;
+            if (i & 1) copy_tile<T, DP, kCols>(dst, (const T*)a.go + tok * a.go_st + head * a.go_sh, a.go_st, t.nb - c0, a.D, tid);
+            else copy_tile<T, DP, kCols>(dst, (const T*)a.q + tok * a.q_st + head * a.q_sh, a.q_st, t.nb - c0, a.D, tid);
+            const float* from = (i & 1 ? a.delta : a.lse2) + (int64_t)head * a.Tq + tok;
+            static_assert(kCols == kCopyThreads, "one statistic per copy thread");
+            cp_async4(base + W::stats + (s * kCols + tid) * 4, c0 + tid < t.nb ? from + tid : a.lse2, c0 + tid < t.nb);
+          } else {
+            if (i & 1) copy_tile<T, DP, kCols>(dst, vp + tok * a.v_st, a.v_st, t.nb - c0, a.D, tid);
+            else copy_tile<T, DP, kCols>(dst, kp + tok * a.k_st, a.k_st, t.nb - c0, a.D, tid);
+          }
+          if (i & 1) {
+            if (++step == per_head) step = 0, ++h;
+          }
+          ring.announce(i);
         }
-        cp_async_commit();
-        cp_async_wait<1>();
-        announce(i);
+        cp_async_wait_all();
       }
-      cp_async_wait<0>();
-      announce(2 * n);
-    }
-  } else if (warp == kMmaWarp) {
-    if (threadIdx.x % 32 == 0 && n > 0) {
-      constexpr uint32_t id_s = mma_desc<T>(kTile, kTile, false), id_o = mma_desc<T>(kTile, DP, true);
-      auto wait_tile = [&](int i) { bar_wait(b_full + 8 * (i % ST), (i / ST) & 1, abort, err); };
-      auto release = [&](int i) {
-        if (i + ST < 2 * n) mma_commit(b_empty + 8 * (i % ST));
+    } else if (warp == kMmaWarp && threadIdx.x % 32 == 0 && n > 0) {
+      // ---- products ----
+      auto y_of = [&](int i) { return sy + (i % ST) * W::tile; };
+      auto score = [&](int j) {
+        ring.wait_operand(2 * j);
+        mma_nt<T, DP, kCols>(tmem + (j % GROUPS) * 128, sx1, y_of(2 * j));
+        mma_commit(b_s + 8 * (j % GROUPS));
       };
-      auto nt = [&](uint32_t d, uint32_t x, int i) {  // d = x y_i^T
-        const uint32_t y = sy + (i % ST) * Sm::tile;
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) {
-          const uint32_t at = (ks / 4) * kPanel + (ks % 4) * 32;
-          mma_ss(d, smem_desc(x + at, 16), smem_desc(y + at, 16), id_s, ks > 0);
-        }
-      };
-      auto add = [&](uint32_t d, uint32_t p, int i, bool more) {  // d (+)= p y_i
-        const uint32_t y = sy + (i % ST) * Sm::tile;
-#pragma unroll
-        for (int ks = 0; ks < kTile / 16; ++ks)
-          mma_ts(d, p + (ks / 4) * 64 + (ks % 4) * 8, smem_desc(y + ks * 16 * kPanelRow, kPanel), id_o, more || ks > 0);
+      auto dscore = [&](int j) {
+        ring.wait_operand(2 * j + 1);
+        mma_nt<T, DP, kCols>(tmem + (j % GROUPS) * 128 + 64, sx2, y_of(2 * j + 1));
+        mma_commit(b_dp + 8 * (j % GROUPS));
+        if (!DKV) ring.release(2 * j + 1);
       };
       bar_wait(b_x, 0, abort, err);
-      wait_tile(0);
-      nt(t_s, sx, 0);
-      mma_commit(b_s);
-      wait_tile(1);
-      nt(t_dp, sx + Sm::tile, 1);
-      mma_commit(b_dp);
-      if (!DKV) release(1);
+      for (int j = 0; j < GROUPS && j < n; ++j) {
+        score(j);
+        dscore(j);
+      }
       for (int j = 0; j < n; ++j) {
-        const int i1 = 2 * j, i2 = 2 * j + 1;
-        bar_wait(b_p, j & 1, abort, err);
+        const int g = j % GROUPS, parity = (j / GROUPS) & 1;
+        bar_wait(b_p + 8 * g, parity, abort, err);
         tc_fence_after();
-        if (DKV) add(t_2, t_s, i2, j > 0);
-        if (j + 1 < n) {
-          wait_tile(i1 + 2);
-          nt(t_s, sx, i1 + 2);
-          mma_commit(b_s);
-        }
-        bar_wait(b_ds, j & 1, abort, err);
+        if (DKV) mma_nn<T, DP, kCols>(t_2, tmem + g * 128, y_of(2 * j + 1), j > 0);
+        if (j + GROUPS < n) score(j + GROUPS);
+        bar_wait(b_ds + 8 * g, parity, abort, err);
         tc_fence_after();
-        add(t_1, t_dp, i1, j > 0);
-        release(i1);
-        if (DKV) release(i2);  // not before: the threads read delta from it
-        if (j + 1 < n) {
-          wait_tile(i2 + 2);
-          nt(t_dp, sx + Sm::tile, i2 + 2);
-          mma_commit(b_dp);
-          if (!DKV) release(i2 + 2);
-        }
+        mma_nn<T, DP, kCols>(t_1, tmem + g * 128 + 64, y_of(2 * j), j > 0);
+        ring.release(2 * j);
+        if (DKV) ring.release(2 * j + 1);  // not before: the threads read delta from it
+        if (j + GROUPS < n) dscore(j + GROUPS);
       }
       mma_commit(b_done);
     }
-    __syncwarp();
-  }
   } else {
-    draw_registers<kRowRegs>();
-    const int half = warp / 4, row = threadIdx.x % kTile;
+    draw_registers<W::row_regs>();
+    const int g = warp / 4, row = threadIdx.x % kTile;
     const uint32_t lane = (uint32_t)(warp % 4) * 32 << 16;
-    const uint32_t ts = t_s + half * 64 + lane, tdp = t_dp + half * 64 + lane;
+    const uint32_t ts = tmem + g * 128 + lane, tdp = ts + 64;
     const bool live = row < t.rows;
     const float qscale = a.scale * kLog2e;
     float c = 1.f;
@@ -551,23 +557,24 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_bwd_kernel(const Packe
       row_lse = a.lse2[(int64_t)head0 * a.Tq + t.row0 + row];
       row_delta = a.delta[(int64_t)head0 * a.Tq + t.row0 + row];
     }
-    // one step's half row: P from S, then dS from dP
+    // one step's row: P from S, then dS from dP
     auto step_rows = [&](int j, int lo, int hi, auto masked) {
       constexpr bool MASK = decltype(masked)::value;
+      const int parity = (j / GROUPS) & 1;
       const u64 q2 = pk(qscale, qscale);
       u64 p[32];
       {
-        const float* lse = stats + ((2 * j) % ST) * kTile + half * 64;  // base 2, negated below
+        const float* lse = stats + ((2 * j) % ST) * kCols;
         uint32_t v[2][32];
-        bar_wait(b_s, j & 1, abort, err);
-        if (DKV) bar_wait(b_full + 8 * ((2 * j) % ST), (2 * j / ST) & 1, abort, err);
+        bar_wait(b_s + 8 * g, parity, abort, err);
+        if (DKV) ring.wait_full(2 * j);
         tc_fence_after();
         tmem_ld32(ts, v[0]);
         tmem_ld32(ts + 32, v[1]);
         tmem_wait_ld();
         if (!DKV) {  // S is read: the next product may overwrite it
           tc_fence_before();
-          bar_arrive(b_p);
+          bar_arrive(b_p + 8 * g);
         }
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
@@ -601,11 +608,11 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_bwd_kernel(const Packe
         tmem_st32(ts, o);
         tmem_wait_st();
         tc_fence_before();
-        bar_arrive(b_p);
+        bar_arrive(b_p + 8 * g);
       }
-      const float* delta = stats + ((2 * j + 1) % ST) * kTile + half * 64;
-      bar_wait(b_dp, j & 1, abort, err);
-      if (DKV) bar_wait(b_full + 8 * ((2 * j + 1) % ST), ((2 * j + 1) / ST) & 1, abort, err);
+      const float* delta = stats + ((2 * j + 1) % ST) * kCols;
+      bar_wait(b_dp + 8 * g, parity, abort, err);
+      if (DKV) ring.wait_full(2 * j + 1);
       tc_fence_after();
       uint32_t v[2][32], o[32];
       tmem_ld32(tdp, v[0]);
@@ -636,58 +643,50 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_bwd_kernel(const Packe
       tmem_st32(tdp, o);
       tmem_wait_st();
       tc_fence_before();
-      bar_arrive(b_ds);
+      bar_arrive(b_ds + 8 * g);
     };
-    int step = 0;
-    for (int j = 0; j < n; ++j) {
-      const int64_t c0 = c_begin + (int64_t)step * kTile + half * 64;
-      if (++step == per_head) step = 0;
-      // columns [lo, hi) of this half that the row meets.  Keys beyond the cloud's end
-      // must not reach dS (their P is unbounded); queries beyond it have zero rows
-      // of Q and dO and lse 0, so they add nothing.
-      int lo = 0, hi = 64;
+    int step = per_head > 0 ? g % per_head : 0;
+    for (int j = g; j < n; j += GROUPS) {
+      const int64_t c0 = c_begin + (int64_t)step * kCols;
+      for (step += GROUPS; step >= per_head;) step -= per_head;
+      // columns [lo, hi) that the row meets.  Keys beyond the cloud's end must not
+      // reach dS (their P is unbounded); queries beyond it have zero rows of Q and dO
+      // and lse 0, so they add nothing.
+      int lo = 0, hi = kCols;
       if (DKV) {
-        if (a.causal) lo = (int)min64(64, max64(0, first + row - shift - c0));
+        if (a.causal) lo = (int)min64(kCols, max64(0, first + row - shift - c0));
       } else {
         int64_t end = t.nb;
         if (a.causal) end = min64(end, first + row + shift + 1);
-        hi = (int)min64(64, max64(0, end - c0));
+        hi = (int)min64(kCols, max64(0, end - c0));
       }
-      const bool whole = __all_sync(0xffffffffu, lo == 0 && hi == 64);
-      if (whole) step_rows(j, lo, hi, std::false_type{});
+      if (__all_sync(0xffffffffu, lo == 0 && hi == kCols)) step_rows(j, lo, hi, std::false_type{});
       else step_rows(j, lo, hi, std::true_type{});
     }
     if (n > 0) {
       bar_wait(b_done, 0, abort, err);
       tc_fence_after();
     }
-    // DKV: the first four warps store dK, the others dV; else each half of the columns
+    // two groups: DKV: the first stores dK, the second dV; else half of the columns each
     const int64_t at = DKV ? ((t.row0 + row) * a.Hk + kvh) * a.D : ((t.row0 + row) * a.H + head0) * a.D;
-    T* op = (T*)(DKV ? (half ? a.dv : a.dk) : a.dq) + at;
-    const float f = DKV && half ? 1.f : a.scale / c;
-    const uint32_t from = (DKV && half ? t_2 : t_1) + lane;
 #pragma unroll
-    for (int x = 0; x < DP; x += 32) {
-      if (!DKV && (x / 32) % 2 != half) continue;
-      uint32_t v[32];
-      if (n > 0) {
-        tmem_ld32(from + x, v);
-        tmem_wait_ld();
-      } else {
+    for (int which = 0; which < (DKV ? 2 : 1); ++which) {
+      if (DKV && GROUPS == 2 && which != g) continue;
+      T* op = (T*)(DKV ? (which ? a.dv : a.dk) : a.dq) + at;
+      const float f = which ? 1.f : a.scale / c;
+      const uint32_t from = (which ? t_2 : t_1) + lane;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = 0;
-      }
-      if (live) {
+      for (int x = 0; x < DP; x += 32) {
+        if (!DKV && GROUPS == 2 && (x / 32) % 2 != g) continue;
+        uint32_t v[32];
+        if (n > 0) {
+          tmem_ld32(from + x, v);
+          tmem_wait_ld();
+        } else {
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-          if (x + i >= a.D) continue;
-          uint4 o;
-          uint32_t* ov = reinterpret_cast<uint32_t*>(&o);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            ov[e] = pack2<T>(__uint_as_float(v[i + 2 * e]) * f, __uint_as_float(v[i + 2 * e + 1]) * f);
-          *reinterpret_cast<uint4*>(op + x + i) = o;
+          for (int i = 0; i < 32; ++i) v[i] = 0;
         }
+        if (live) store32<T>(op, v, f, x, a.D);
       }
     }
     tc_fence_before();
@@ -695,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, 1) packed_mma_bwd_kernel(const Packe
   __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after();
-    tmem_free(tmem, 512);
+    tmem_free(tmem, W::tmem);
   }
 }
 
@@ -706,28 +705,29 @@ int set_smem(K kern, int bytes) {
 
 template <typename T, int DP>
 int fwd(const PackedArgs& a, cudaStream_t st) {
+  using F = Fwd<DP>;
   auto kern = packed_mma_fwd_kernel<T, DP>;
-  int s = set_smem(kern, FwdSmem<DP>::total);
+  int s = set_smem(kern, F::smem);
   if (s) return s;
-  kern<<<dim3((unsigned)packed_slots(a.Tq, a.B, 2 * kTile), a.H), kThreads, FwdSmem<DP>::total, st>>>(a);
+  kern<<<dim3((unsigned)packed_slots(a.Tq, a.B, F::TILES * kTile), a.H), F::threads, F::smem, st>>>(a);
   return check_launch();
 }
 
 template <typename T, int DP>
 int bwd(const PackedArgs& a, cudaStream_t st) {
-  constexpr int smem = BwdSmem<DP>::total;
+  using W = Bwd<DP>;
   if (a.dk && a.Tk > 0) {
     auto kern = packed_mma_bwd_kernel<T, DP, true>;
-    int s = set_smem(kern, smem);
+    int s = set_smem(kern, W::smem);
     if (s) return s;
-    kern<<<dim3((unsigned)packed_slots(a.Tk, a.B, kTile), a.Hk), kThreads, smem, st>>>(a);
+    kern<<<dim3((unsigned)packed_slots(a.Tk, a.B, kTile), a.Hk), W::threads, W::smem, st>>>(a);
     if ((s = check_launch())) return s;
   }
   if (a.dq && a.Tq > 0) {
     auto kern = packed_mma_bwd_kernel<T, DP, false>;
-    int s = set_smem(kern, smem);
+    int s = set_smem(kern, W::smem);
     if (s) return s;
-    kern<<<dim3((unsigned)packed_slots(a.Tq, a.B, kTile), a.H), kThreads, smem, st>>>(a);
+    kern<<<dim3((unsigned)packed_slots(a.Tq, a.B, kTile), a.H), W::threads, W::smem, st>>>(a);
     if ((s = check_launch())) return s;
   }
   return TPO_OK;

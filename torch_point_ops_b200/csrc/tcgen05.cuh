@@ -43,17 +43,24 @@ __device__ __forceinline__ void bar_wait(uint32_t bar, uint32_t parity, volatile
   atomicOr(err, kErrMmaTimeout);
 }
 
-#ifndef CPH
-#define CPH ""
-#endif
 // ---- 16-byte asynchronous copies; a false predicate writes zeros ----
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool read) {
-  asm volatile("cp.async.cg.shared.global" CPH " [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(read ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-// generic-proxy writes of this thread become visible to the tensor core's reads
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool read) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(read ? 4 : 0) : "memory");
+}
+// arrives on the mbarrier once every copy that this thread issued before has landed
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// orders generic-proxy accesses to shared memory (this thread's, and those it has
+// synchronised with) before later asynchronous-proxy ones: the tensor
+// core's reads see the writes
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // ---- tensor memory ----

@@ -21,39 +21,51 @@ constexpr int kCopyThreads = 64;
 
 // ROWS rows of a packed tensor into a swizzled tile, by the copy warps (t = index).
 // Rows at or beyond `valid` and columns at or beyond D become zeros: nothing from
-// another cloud enters a product (0 * NaN would).
+// another cloud enters a product (0 * NaN would).  A whole tile takes an address
+// addition and a copy per 16 bytes: two warps have to keep up with the tensor core.
 template <typename T, int DP, int ROWS>
 __device__ __forceinline__ void copy_tile(uint32_t dst, const T* src, int64_t stride, int64_t valid, int D, int t) {
   constexpr int CH = DP / 8;               // 16-byte chunks per row
-  constexpr int STEP = kCopyThreads / CH;  // rows per pass
+  constexpr int STEP = kCopyThreads / CH;  // rows per pass: 4 or 8
   const int c = t % CH, r0 = t / CH;
-  const uint32_t at = dst + (c >> 3) * ROWS * kPanelRow;
   const bool col = c * 8 < D;
-  const T* p = src + (int64_t)r0 * stride + c * 8;
-#pragma unroll 8
-  for (int r = r0; r < ROWS; r += STEP) {
-    const bool in = col && r < valid;
-    cp_async16(at + r * kPanelRow + (((c & 7) ^ (r & 7)) << 4), in ? (const void*)p : (const void*)src, in);
-    p += STEP * stride;
+  const uint32_t at = dst + (c >> 3) * ROWS * kPanelRow + r0 * kPanelRow;
+  // the swizzle depends on the row modulo 8: the same in every second pass
+  const uint32_t even = at + (((c & 7) ^ (r0 & 7)) << 4), odd = at + (((c & 7) ^ ((r0 + STEP) & 7)) << 4);
+  const T* p = src + (int64_t)r0 * stride + (col ? c * 8 : 0);
+  const int64_t hop = STEP * stride;
+  if (valid >= ROWS) {
+#pragma unroll
+    for (int i = 0; i < ROWS / STEP; ++i) {
+      cp_async16((i & 1 ? odd : even) + i * STEP * kPanelRow, p, col);
+      p += hop;
+    }
+  } else {
+#pragma unroll 4
+    for (int i = 0; i < ROWS / STEP; ++i) {
+      const bool in = r0 + i * STEP < valid;
+      cp_async16((i & 1 ? odd : even) + i * STEP * kPanelRow, in ? p : src, in && col);
+      p += hop;
+    }
   }
 }
 
 // d (+)= x y^T over the width: x 128 rows, y NY rows, both K-major.
 template <typename T, int DP, int NY>
-__device__ __forceinline__ void mma_nt(uint32_t d, uint32_t x, uint32_t y) {
+__device__ __forceinline__ void mma_nt(uint32_t lane, uint32_t d, uint32_t x, uint32_t y) {
   constexpr uint32_t id = mma_desc<T>(kTile, NY, false);
 #pragma unroll
   for (int ks = 0; ks < DP / 16; ++ks)
-    mma_ss(d, smem_desc(x + (ks / 4) * kTile * kPanelRow + (ks % 4) * 32, 16),
+    mma_ss(lane, d, smem_desc(x + (ks / 4) * kTile * kPanelRow + (ks % 4) * 32, 16),
            smem_desc(y + (ks / 4) * NY * kPanelRow + (ks % 4) * 32, 16), id, ks > 0);
 }
 // d (+)= p y over y's NY rows: p 128 rows of 16-bit values in TMEM, y MN-major.
 template <typename T, int DP, int NY>
-__device__ __forceinline__ void mma_nn(uint32_t d, uint32_t p, uint32_t y, bool more) {
+__device__ __forceinline__ void mma_nn(uint32_t lane, uint32_t d, uint32_t p, uint32_t y, bool more) {
   constexpr uint32_t id = mma_desc<T>(kTile, DP, true);
 #pragma unroll
   for (int ks = 0; ks < NY / 16; ++ks)
-    mma_ts(d, p + ks * 8, smem_desc(y + ks * 16 * kPanelRow, NY * kPanelRow), id, more || ks > 0);
+    mma_ts(lane, d, p + ks * 8, smem_desc(y + ks * 16 * kPanelRow, NY * kPanelRow), id, more || ks > 0);
 }
 
 // 32 accumulator columns times f as 16-bit values to global memory, whole chunks of 8.
@@ -91,8 +103,8 @@ struct Ring {
     wait_full(i);
     fence_async_smem();
   }
-  __device__ __forceinline__ void release(int i) const {
-    if (i + ST < tiles) mma_commit(empty + 8 * (i % ST));
+  __device__ __forceinline__ void release(uint32_t lane, int i) const {
+    if (i + ST < tiles) mma_commit(lane, empty + 8 * (i % ST));
   }
 };
 
@@ -202,27 +214,29 @@ __global__ void __launch_bounds__(Fwd<DP>::threads, Fwd<DP>::TILES == 2 ? 1 : 2)
         }
         cp_async_wait_all();
       }
-    } else if (warp == kMmaWarp && threadIdx.x % 32 == 0 && n > 0) {
-      // ---- products ----
+    } else if (warp == kMmaWarp && n > 0) {
+      // ---- products: the warp stays together, one lane issues ----
+      const uint32_t one = elect_lane();
+      const uint32_t u_s = uniform(t_s), u_p = uniform(t_p), u_o = uniform(t_o), u_q = uniform(sq);
       auto score = [&](int w, int j) {  // S_w = Q_w K_j^T
-        mma_nt<T, DP, kTile>(t_s + w * kTile, sq + w * F::tile, skv + ((2 * j) % ST) * F::tile);
-        mma_commit(b_s + 8 * w);
+        mma_nt<T, DP, kTile>(one, u_s + w * kTile, u_q + w * F::tile, uniform(skv + ((2 * j) % ST) * F::tile));
+        mma_commit(one, b_s + 8 * w);
       };
       bar_wait(b_q, 0, abort, err);
       ring.wait_operand(0);
 #pragma unroll
       for (int w = 0; w < TILES; ++w)
         if (steps[w] > 0) score(w, 0);
-      ring.release(0);
+      ring.release(one, 0);
       for (int j = 0; j < n; ++j) {
         const int iv = 2 * j + 1, ik = 2 * j + 2;
-        const uint32_t v = skv + (iv % ST) * F::tile;
+        const uint32_t v = uniform(skv + (iv % ST) * F::tile);
         if (F::APART && j + 1 < n) {
           bar_wait(b_read, j & 1, abort, err);
           tc_fence_after();
           ring.wait_operand(ik);
           score(0, j + 1);
-          ring.release(ik);
+          ring.release(one, ik);
         }
         ring.wait_operand(iv);
         if (!F::APART && j + 1 < n) ring.wait_operand(ik);
@@ -231,12 +245,12 @@ __global__ void __launch_bounds__(Fwd<DP>::threads, Fwd<DP>::TILES == 2 ? 1 : 2)
           if (j >= steps[w]) continue;
           bar_wait(b_p + 8 * w, j & 1, abort, err);
           tc_fence_after();
-          mma_nn<T, DP, kTile>(t_o + w * DP, t_p + w * kTile, v, j > 0);
-          if (F::APART || j + 1 == steps[w]) mma_commit(b_o + 8 * w);
+          mma_nn<T, DP, kTile>(one, u_o + w * DP, u_p + w * kTile, v, j > 0);
+          if (F::APART || j + 1 == steps[w]) mma_commit(one, b_o + 8 * w);
           else score(w, j + 1);
         }
-        ring.release(iv);
-        if (!F::APART) ring.release(ik);
+        ring.release(one, iv);
+        if (!F::APART) ring.release(one, ik);
       }
     }
   } else {
@@ -497,19 +511,22 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
         }
         cp_async_wait_all();
       }
-    } else if (warp == kMmaWarp && threadIdx.x % 32 == 0 && n > 0) {
-      // ---- products ----
-      auto y_of = [&](int i) { return sy + (i % ST) * W::tile; };
+    } else if (warp == kMmaWarp && n > 0) {
+      // ---- products: the warp stays together, one lane issues ----
+      const uint32_t one = elect_lane();
+      const uint32_t u_tmem = uniform(tmem), u_x1 = uniform(sx1), u_x2 = uniform(sx2);
+      auto y_of = [&](int i) { return uniform(sy + (i % ST) * W::tile); };
+      auto s_of = [&](int j) { return GROUPS == 1 ? u_tmem : uniform(tmem + (j % GROUPS) * 128); };
       auto score = [&](int j) {
         ring.wait_operand(2 * j);
-        mma_nt<T, DP, kCols>(tmem + (j % GROUPS) * 128, sx1, y_of(2 * j));
-        mma_commit(b_s + 8 * (j % GROUPS));
+        mma_nt<T, DP, kCols>(one, s_of(j), u_x1, y_of(2 * j));
+        mma_commit(one, b_s + 8 * (j % GROUPS));
       };
       auto dscore = [&](int j) {
         ring.wait_operand(2 * j + 1);
-        mma_nt<T, DP, kCols>(tmem + (j % GROUPS) * 128 + 64, sx2, y_of(2 * j + 1));
-        mma_commit(b_dp + 8 * (j % GROUPS));
-        if (!DKV) ring.release(2 * j + 1);
+        mma_nt<T, DP, kCols>(one, s_of(j) + 64, u_x2, y_of(2 * j + 1));
+        mma_commit(one, b_dp + 8 * (j % GROUPS));
+        if (!DKV) ring.release(one, 2 * j + 1);
       };
       bar_wait(b_x, 0, abort, err);
       for (int j = 0; j < GROUPS && j < n; ++j) {
@@ -520,16 +537,16 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
         const int g = j % GROUPS, parity = (j / GROUPS) & 1;
         bar_wait(b_p + 8 * g, parity, abort, err);
         tc_fence_after();
-        if (DKV) mma_nn<T, DP, kCols>(t_2, tmem + g * 128, y_of(2 * j + 1), j > 0);
+        if (DKV) mma_nn<T, DP, kCols>(one, u_tmem + W::acc2, s_of(j), y_of(2 * j + 1), j > 0);
         if (j + GROUPS < n) score(j + GROUPS);
         bar_wait(b_ds + 8 * g, parity, abort, err);
         tc_fence_after();
-        mma_nn<T, DP, kCols>(t_1, tmem + g * 128 + 64, y_of(2 * j), j > 0);
-        ring.release(2 * j);
-        if (DKV) ring.release(2 * j + 1);  // not before: the threads read delta from it
+        mma_nn<T, DP, kCols>(one, u_tmem + W::acc1, s_of(j) + 64, y_of(2 * j), j > 0);
+        ring.release(one, 2 * j);
+        if (DKV) ring.release(one, 2 * j + 1);  // not before: the threads read delta from it
         if (j + GROUPS < n) dscore(j + GROUPS);
       }
-      mma_commit(b_done);
+      mma_commit(one, b_done);
     }
   } else {
     draw_registers<W::row_regs>();

@@ -217,9 +217,11 @@ __global__ void __launch_bounds__(Fwd<DP>::threads, Fwd<DP>::TILES == 2 ? 1 : 2)
     } else if (warp == kMmaWarp && n > 0) {
       // ---- products: the warp stays together, one lane issues ----
       const uint32_t one = elect_lane();
-      const uint32_t u_s = uniform(t_s), u_p = uniform(t_p), u_o = uniform(t_o), u_q = uniform(sq);
+      const uint32_t u_tmem = uniform(tmem), u_base = uniform(base);
+      const uint32_t u_s = u_tmem + F::s, u_p = u_tmem + F::p, u_o = u_tmem + F::o, u_q = u_base, u_kv = u_base + TILES * F::tile;
+      const int un = (int)uniform(n);  // loops and stages count in uniform registers too
       auto score = [&](int w, int j) {  // S_w = Q_w K_j^T
-        mma_nt<T, DP, kTile>(one, u_s + w * kTile, u_q + w * F::tile, uniform(skv + ((2 * j) % ST) * F::tile));
+        mma_nt<T, DP, kTile>(one, u_s + w * kTile, u_q + w * F::tile, u_kv + ((2 * j) % ST) * F::tile);
         mma_commit(one, b_s + 8 * w);
       };
       bar_wait(b_q, 0, abort, err);
@@ -228,10 +230,10 @@ __global__ void __launch_bounds__(Fwd<DP>::threads, Fwd<DP>::TILES == 2 ? 1 : 2)
       for (int w = 0; w < TILES; ++w)
         if (steps[w] > 0) score(w, 0);
       ring.release(one, 0);
-      for (int j = 0; j < n; ++j) {
+      for (int j = 0; j < un; ++j) {
         const int iv = 2 * j + 1, ik = 2 * j + 2;
-        const uint32_t v = uniform(skv + (iv % ST) * F::tile);
-        if (F::APART && j + 1 < n) {
+        const uint32_t v = u_kv + (iv % ST) * F::tile;
+        if (F::APART && j + 1 < un) {
           bar_wait(b_read, j & 1, abort, err);
           tc_fence_after();
           ring.wait_operand(ik);
@@ -239,7 +241,7 @@ __global__ void __launch_bounds__(Fwd<DP>::threads, Fwd<DP>::TILES == 2 ? 1 : 2)
           ring.release(one, ik);
         }
         ring.wait_operand(iv);
-        if (!F::APART && j + 1 < n) ring.wait_operand(ik);
+        if (!F::APART && j + 1 < un) ring.wait_operand(ik);
 #pragma unroll
         for (int w = 0; w < TILES; ++w) {
           if (j >= steps[w]) continue;
@@ -423,7 +425,7 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
   const uint32_t sx1 = base, sx2 = base + W::own, sy = base + 2 * W::own, bars = base + W::bars;
   const float* stats = reinterpret_cast<const float*>(smem_raw + (base + W::stats - raw));
   const uint32_t b_x = bars, b_full = bars + 8, b_empty = b_full + 8 * ST, b_s = b_empty + 8 * ST, b_dp = b_s + 16,
-                 b_p = b_dp + 16, b_ds = b_p + 16, b_done = b_ds + 16, s_tmem = b_done + 8, s_abort = s_tmem + 4;
+                 b_p = b_dp + 16, b_ds = b_p + 16, b_used1 = b_ds + 16, b_used2 = b_used1 + 16, b_done = b_used2 + 16, s_tmem = b_done + 8, s_abort = s_tmem + 4;
   volatile int* abort = reinterpret_cast<volatile int*>(smem_raw + (s_abort - raw));
   unsigned* err = &g_attention_error;
 
@@ -455,6 +457,8 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
         bar_init(b_dp + 8 * g, 1);
         bar_init(b_p + 8 * g, 128);
         bar_init(b_ds + 8 * g, 128);
+        bar_init(b_used1 + 8 * g, 1);
+        bar_init(b_used2 + 8 * g, 1);
       }
       bar_init(b_done, 1);
       *abort = 0;
@@ -511,42 +515,56 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
         }
         cp_async_wait_all();
       }
-    } else if (warp == kMmaWarp && n > 0) {
-      // ---- products: the warp stays together, one lane issues ----
+    } else if (n > 0) {
+      // ---- products: a warp stays together, one lane issues.  One warp computes S and dP, the other
+      // dK and dV or dQ: waiting on a barrier costs some 130 clocks even when it is open,
+      // and one warp alone would spend more on its four waits per tile than the products take.
       const uint32_t one = elect_lane();
-      const uint32_t u_tmem = uniform(tmem), u_x1 = uniform(sx1), u_x2 = uniform(sx2);
-      auto y_of = [&](int i) { return uniform(sy + (i % ST) * W::tile); };
-      auto s_of = [&](int j) { return GROUPS == 1 ? u_tmem : uniform(tmem + (j % GROUPS) * 128); };
-      auto score = [&](int j) {
-        ring.wait_operand(2 * j);
-        mma_nt<T, DP, kCols>(one, s_of(j), u_x1, y_of(2 * j));
-        mma_commit(one, b_s + 8 * (j % GROUPS));
-      };
-      auto dscore = [&](int j) {
-        ring.wait_operand(2 * j + 1);
-        mma_nt<T, DP, kCols>(one, s_of(j) + 64, u_x2, y_of(2 * j + 1));
-        mma_commit(one, b_dp + 8 * (j % GROUPS));
-        if (!DKV) ring.release(one, 2 * j + 1);
-      };
-      bar_wait(b_x, 0, abort, err);
-      for (int j = 0; j < GROUPS && j < n; ++j) {
-        score(j);
-        dscore(j);
+      const uint32_t u_tmem = uniform(tmem), u_x1 = uniform(base), u_x2 = u_x1 + W::own, u_y = u_x1 + 2 * W::own;
+      const int un = (int)uniform(n);  // loops and stages count in uniform registers too
+      auto y_of = [&](int i) { return u_y + (i % ST) * W::tile; };
+      auto s_of = [&](int j) { return u_tmem + (j % GROUPS) * 128; };
+      if (warp == kMmaWarp) {
+        bar_wait(b_x, 0, abort, err);
+        fence_async_smem();
+        for (int j = 0; j < un; ++j) {
+          const int g = j % GROUPS, parity = (j / GROUPS - 1) & 1;
+          ring.wait_operand(2 * j);
+          if (j >= GROUPS) {  // S of the tile before is read (DKV: and its P has been multiplied)
+            bar_wait((DKV ? b_used2 : b_p) + 8 * g, parity, abort, err);
+            tc_fence_after();
+          }
+          mma_nt<T, DP, kCols>(one, s_of(j), u_x1, y_of(2 * j));
+          mma_commit(one, b_s + 8 * g);
+          ring.wait_operand(2 * j + 1);
+          if (j >= GROUPS) {  // dS of the tile before has been multiplied
+            bar_wait(b_used1 + 8 * g, parity, abort, err);
+            tc_fence_after();
+          }
+          mma_nt<T, DP, kCols>(one, s_of(j) + 64, u_x2, y_of(2 * j + 1));
+          mma_commit(one, b_dp + 8 * g);
+          if (!DKV) ring.release(one, 2 * j + 1);
+        }
+      } else {
+        for (int j = 0; j < un; ++j) {
+          const int g = j % GROUPS, parity = (j / GROUPS) & 1;
+          if (DKV) {
+            bar_wait(b_p + 8 * g, parity, abort, err);
+            tc_fence_after();
+            fence_async_smem();  // the copies landed before S was computed
+            mma_nn<T, DP, kCols>(one, u_tmem + W::acc2, s_of(j), y_of(2 * j + 1), j > 0);
+            if (j + GROUPS < un) mma_commit(one, b_used2 + 8 * g);
+          }
+          bar_wait(b_ds + 8 * g, parity, abort, err);
+          tc_fence_after();
+          fence_async_smem();
+          mma_nn<T, DP, kCols>(one, u_tmem + W::acc1, s_of(j) + 64, y_of(2 * j), j > 0);
+          if (j + GROUPS < un) mma_commit(one, b_used1 + 8 * g);
+          ring.release(one, 2 * j);
+          if (DKV) ring.release(one, 2 * j + 1);  // not before: the threads read delta from it
+        }
+        mma_commit(one, b_done);
       }
-      for (int j = 0; j < n; ++j) {
-        const int g = j % GROUPS, parity = (j / GROUPS) & 1;
-        bar_wait(b_p + 8 * g, parity, abort, err);
-        tc_fence_after();
-        if (DKV) mma_nn<T, DP, kCols>(one, u_tmem + W::acc2, s_of(j), y_of(2 * j + 1), j > 0);
-        if (j + GROUPS < n) score(j + GROUPS);
-        bar_wait(b_ds + 8 * g, parity, abort, err);
-        tc_fence_after();
-        mma_nn<T, DP, kCols>(one, u_tmem + W::acc1, s_of(j) + 64, y_of(2 * j), j > 0);
-        ring.release(one, 2 * j);
-        if (DKV) ring.release(one, 2 * j + 1);  // not before: the threads read delta from it
-        if (j + GROUPS < n) dscore(j + GROUPS);
-      }
-      mma_commit(one, b_done);
     }
   } else {
     draw_registers<W::row_regs>();

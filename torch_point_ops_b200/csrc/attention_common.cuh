@@ -45,29 +45,43 @@ struct Tile {
 // before the first and after the last offset; nobody attends there.
 inline int64_t packed_slots(int64_t tokens, int64_t clouds, int BM) { return tokens / BM + clouds + 2; }
 
-// All 32 lanes of a warp call this with the same slot.
+// All 32 lanes of a warp call this with the same slot.  With at most 30 clouds every
+// lane holds one start and one round of loads does; else 32 probes a round narrow the range.
 __device__ __forceinline__ Tile find_tile(const int64_t* off, int64_t T, const int64_t* other,
                                           int64_t To, int B, int BM, int64_t slot) {
   const int lane = threadIdx.x & 31;
-  auto start = [&](int i) -> int64_t {  // clamped start of extended cloud i in [0, B + 2]
-    if (i == 0) return 0;
-    if (i == B + 2) return T;
-    return min64(max64(off[i - 1], 0), T);
-  };
-  // greatest i in [lo, hi) with start(i)/BM + i <= slot; 32 probes a step
-  int lo = 0, hi = B + 2;
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32;
-    const int i = lo + lane * step;
-    const bool le = i < hi && (lane == 0 || start(i) / BM + i <= slot);
-    const unsigned m = __ballot_sync(0xffffffffu, le);
-    const int last = 31 - __clz(m);
-    hi = min(hi, lo + (last + 1) * step);
-    lo += last * step;
+  // clamped start of extended cloud i in [0, B + 2], from its raw offset
+  auto start = [&](int i, int64_t raw) -> int64_t { return i == 0 ? 0 : i >= B + 2 ? T : min64(max64(raw, 0), T); };
+  int lo = 0, lo0 = 0;  // lane k holds the offsets of cloud lo0 + k
+  int64_t raw = 0, raw_other = 0;
+  if (B + 2 <= 31) {
+    const bool in = lane >= 1 && lane <= B + 1;
+    raw = in ? off[lane - 1] : 0;
+    raw_other = in ? other[lane - 1] : 0;
+    const unsigned m = __ballot_sync(0xffffffffu, lane < B + 2 && (lane == 0 || start(lane, raw) / BM + lane <= slot));
+    lo = 31 - __clz(m);
+  } else {
+    int hi = B + 2;
+    while (hi - lo > 1) {  // greatest i in [lo, hi) with start(i)/BM + i <= slot
+      const int width = (hi - lo + 31) / 32;
+      const int i = lo + lane * width;
+      const bool le = i < hi && (lane == 0 || start(i, i >= 1 && i <= B + 1 ? off[i - 1] : 0) / BM + i <= slot);
+      const unsigned m = __ballot_sync(0xffffffffu, le);
+      const int last = 31 - __clz(m);
+      hi = min(hi, lo + (last + 1) * width);
+      lo += last * width;
+    }
+    lo0 = lo;
+    const int i = lo + lane;
+    const bool in = lane < 2 && i >= 1 && i <= B + 1;
+    raw = in ? off[i - 1] : 0;
+    raw_other = in ? other[i - 1] : 0;
   }
+  const int64_t r0 = __shfl_sync(0xffffffffu, raw, lo - lo0), r1 = __shfl_sync(0xffffffffu, raw, lo - lo0 + 1);
+  const int64_t o0 = __shfl_sync(0xffffffffu, raw_other, lo - lo0), o1 = __shfl_sync(0xffffffffu, raw_other, lo - lo0 + 1);
   Tile t;
-  t.a0 = start(lo);
-  const int64_t end = start(lo + 1);
+  t.a0 = start(lo, r0);
+  const int64_t end = start(lo + 1, r1);
   t.na = max64(end - t.a0, 0);
   t.row0 = t.a0 + (slot - (t.a0 / BM + lo)) * BM;
   t.rows = (int)max64(0, min64(end - t.row0, BM));
@@ -75,10 +89,9 @@ __device__ __forceinline__ Tile find_tile(const int64_t* off, int64_t T, const i
   t.b0 = 0;
   t.nb = 0;
   if (lo >= 1 && lo <= B) {
-    const int64_t r0 = other[lo - 1], r1 = other[lo];
-    t.b0 = min64(max64(r0, 0), To);
-    t.nb = max64(min64(max64(r1, 0), To) - t.b0, 0);
-    if (lane == 0 && (r0 < 0 || r1 < r0 || r1 > To || off[lo - 1] < 0 || off[lo] < off[lo - 1] || off[lo] > T))
+    t.b0 = min64(max64(o0, 0), To);
+    t.nb = max64(min64(max64(o1, 0), To) - t.b0, 0);
+    if (lane == 0 && (o0 < 0 || o1 < o0 || o1 > To || r0 < 0 || r1 < r0 || r1 > T))
       atomicOr(&g_attention_error, kErrBadOffsets);
   }
   return t;

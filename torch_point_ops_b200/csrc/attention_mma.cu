@@ -19,14 +19,14 @@ namespace {
 constexpr int kTile = 128;  // rows of a block's own tiles
 constexpr int kCopyThreads = 64;
 
-// ROWS rows of a packed tensor into a swizzled tile, by the copy warps (t = index).
+// ROWS rows of a packed tensor into a swizzled tile, by THREADS threads (t = index).
 // Rows at or beyond `valid` and columns at or beyond D become zeros: nothing from
 // another cloud enters a product (0 * NaN would).  A whole tile takes an address
 // addition and a copy per 16 bytes: two warps have to keep up with the tensor core.
-template <typename T, int DP, int ROWS>
+template <typename T, int DP, int ROWS, int THREADS = kCopyThreads>
 __device__ __forceinline__ void copy_tile(uint32_t dst, const T* src, int64_t stride, int64_t valid, int D, int t) {
   constexpr int CH = DP / 8;               // 16-byte chunks per row
-  constexpr int STEP = kCopyThreads / CH;  // rows per pass: 4 or 8
+  constexpr int STEP = THREADS / CH;       // rows per pass: 4, 8 or 16
   const int c = t % CH, r0 = t / CH;
   const bool col = c * 8 < D;
   const uint32_t at = dst + (c >> 3) * ROWS * kPanelRow + r0 * kPanelRow;
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(Fwd<DP>::threads, Fwd<DP>::TILES == 2 ? 1 : 2)
   const uint32_t raw = smem_addr(smem_raw);
   const uint32_t base = (raw + 1023) & ~1023u;
   const uint32_t sq = base, skv = base + TILES * F::tile, bars = base + F::bars;
-  const uint32_t b_q = bars, b_full = bars + 8, b_empty = b_full + 8 * ST, b_s = b_empty + 8 * ST, b_p = b_s + 16,
+  const uint32_t b_q = bars, b_full = bars + 16, b_empty = b_full + 8 * ST, b_s = b_empty + 8 * ST, b_p = b_s + 16,
                  b_o = b_p + 16, b_read = b_o + 16, s_tmem = b_read + 16, s_abort = s_tmem + 4;
   volatile int* abort = reinterpret_cast<volatile int*>(smem_raw + (s_abort - raw));
   unsigned* err = &g_attention_error;
@@ -166,12 +166,12 @@ __global__ void __launch_bounds__(Fwd<DP>::threads, Fwd<DP>::TILES == 2 ? 1 : 2)
 
   if (warp == kMmaWarp) {
     if (threadIdx.x % 32 == 0) {
-      bar_init(b_q, kCopyThreads);
       for (int i = 0; i < ST; ++i) {
         bar_init(b_full + 8 * i, kCopyThreads);
         bar_init(b_empty + 8 * i, 1);
       }
       for (int w = 0; w < TILES; ++w) {
+        bar_init(b_q + 8 * w, 128);
         bar_init(b_s + 8 * w, 1);
         bar_init(b_p + 8 * w, 128);
         bar_init(b_o + 8 * w, 1);
@@ -194,14 +194,9 @@ __global__ void __launch_bounds__(Fwd<DP>::threads, Fwd<DP>::TILES == 2 ? 1 : 2)
   if (warp >= kCopyWarp) {
     give_registers<F::other_regs>();
     if (warp < kMmaWarp) {
-      // ---- copies: Q, then K0 V0 K1 V1 ... ----
+      // ---- copies: K0 V0 K1 V1 ... ----
       const int tid = threadIdx.x - 32 * kCopyWarp;
       if (n > 0) {
-        const T* qp = (const T*)a.q + t.row0 * a.q_st + head * a.q_sh;
-#pragma unroll
-        for (int w = 0; w < TILES; ++w)
-          copy_tile<T, DP, kTile>(sq + w * F::tile, qp + (int64_t)w * kTile * a.q_st, a.q_st, t.rows - w * kTile, a.D, tid);
-        cp_async_arrive(b_q);
         const T* kp = (const T*)a.k + t.b0 * a.k_st + kvh * a.k_sh;
         const T* vp = (const T*)a.v + t.b0 * a.v_st + kvh * a.v_sh;
         for (int i = 0; i < 2 * n; ++i) {
@@ -224,11 +219,14 @@ __global__ void __launch_bounds__(Fwd<DP>::threads, Fwd<DP>::TILES == 2 ? 1 : 2)
         mma_nt<T, DP, kTile>(one, u_s + w * kTile, u_q + w * F::tile, u_kv + ((2 * j) % ST) * F::tile);
         mma_commit(one, b_s + 8 * w);
       };
-      bar_wait(b_q, 0, abort, err);
-      ring.wait_operand(0);
+      ring.wait_full(0);
 #pragma unroll
       for (int w = 0; w < TILES; ++w)
-        if (steps[w] > 0) score(w, 0);
+        if (steps[w] > 0) {
+          bar_wait(b_q + 8 * w, 0, abort, err);
+          fence_async_smem();
+          score(w, 0);
+        }
       ring.release(one, 0);
       for (int j = 0; j < un; ++j) {
         const int iv = 2 * j + 1, ik = 2 * j + 2;
@@ -259,13 +257,18 @@ __global__ void __launch_bounds__(Fwd<DP>::threads, Fwd<DP>::TILES == 2 ? 1 : 2)
     // ---- softmax: a thread owns a row ----
     draw_registers<F::row_regs>();
     const int w = warp / 4, row = threadIdx.x % kTile;
+    if (t.rows > w * kTile) {  // its queries
+      copy_tile<T, DP, kTile, 128>(sq + w * F::tile, (const T*)a.q + (t.row0 + w * kTile) * a.q_st + head * a.q_sh, a.q_st,
+                                   t.rows - w * kTile, a.D, row);
+      cp_async_arrive(b_q + 8 * w);
+    }
     const uint32_t lane = (uint32_t)(warp % 4) * 32 << 16;
     const uint32_t ts = t_s + w * kTile + lane, tp = t_p + w * kTile + lane, to = t_o + w * DP + lane;
     const bool live = w * kTile + row < t.rows;
     const float qscale = a.scale * kLog2e;
     const int my_steps = w == 0 ? steps[0] : steps[TILES - 1];
-    // this row sees keys below `sees`
-    const int64_t sees = a.causal ? min64(t.nb, first + w * kTile + row + shift + 1) : t.nb;
+    // this row sees keys below `sees` (tokens fit 31 bits)
+    const int sees = (int)(a.causal ? max64(0, min64(t.nb, first + w * kTile + row + shift + 1)) : t.nb);
     float m = -INFINITY, l = 0.f;
     // one step's row: masked columns count as -inf
     auto step = [&](int j, int lim, auto masked) {
@@ -340,8 +343,7 @@ __global__ void __launch_bounds__(Fwd<DP>::threads, Fwd<DP>::TILES == 2 ? 1 : 2)
       bar_arrive(b_p + 8 * w);
     };
     for (int j = 0; j < my_steps; ++j) {
-      const int64_t left = sees - (int64_t)j * kTile;
-      const int lim = left >= kTile ? kTile : left > 0 ? (int)left : 0;
+      const int lim = min(kTile, max(0, sees - j * kTile));
       const bool whole = __all_sync(0xffffffffu, lim == kTile);
       bar_wait(b_s + 8 * w, j & 1, abort, err);
       tc_fence_after();
@@ -368,6 +370,7 @@ __global__ void __launch_bounds__(Fwd<DP>::threads, Fwd<DP>::TILES == 2 ? 1 : 2)
       }
       if (live) store32<T>(op, v, inv, c, a.D);
     }
+    cp_async_wait_all();
     tc_fence_before();
   }
   __syncthreads();
@@ -680,21 +683,16 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
       tc_fence_before();
       bar_arrive(b_ds + 8 * g);
     };
+    // Columns [lo, hi) of a tile that the row meets.  Keys beyond the cloud's end must not
+    // reach dS (their P is unbounded); queries beyond it have zero rows of Q and dO and
+    // lse 0, so they add nothing.  Counted from c_begin: fits 31 bits.
+    const int from = DKV && a.causal ? (int)max64(0, first + row - shift - c_begin) : 0;
+    const int to = DKV ? 0 : (int)(a.causal ? max64(0, min64(t.nb, first + row + shift + 1)) : t.nb);
     int step = per_head > 0 ? g % per_head : 0;
     for (int j = g; j < n; j += GROUPS) {
-      const int64_t c0 = c_begin + (int64_t)step * kCols;
+      const int lo = DKV ? min(kCols, max(0, from - step * kCols)) : 0;
+      const int hi = DKV ? kCols : min(kCols, max(0, to - step * kCols));
       for (step += GROUPS; step >= per_head;) step -= per_head;
-      // columns [lo, hi) that the row meets.  Keys beyond the cloud's end must not
-      // reach dS (their P is unbounded); queries beyond it have zero rows of Q and dO
-      // and lse 0, so they add nothing.
-      int lo = 0, hi = kCols;
-      if (DKV) {
-        if (a.causal) lo = (int)min64(kCols, max64(0, first + row - shift - c0));
-      } else {
-        int64_t end = t.nb;
-        if (a.causal) end = min64(end, first + row + shift + 1);
-        hi = (int)min64(kCols, max64(0, end - c0));
-      }
       if (__all_sync(0xffffffffu, lo == 0 && hi == kCols)) step_rows(j, lo, hi, std::false_type{});
       else step_rows(j, lo, hi, std::true_type{});
     }
@@ -709,13 +707,13 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
       if (DKV && GROUPS == 2 && which != g) continue;
       T* op = (T*)(DKV ? (which ? a.dv : a.dk) : a.dq) + at;
       const float f = which ? 1.f : a.scale / c;
-      const uint32_t from = (which ? t_2 : t_1) + lane;
+      const uint32_t acc = (which ? t_2 : t_1) + lane;
 #pragma unroll
       for (int x = 0; x < DP; x += 32) {
         if (!DKV && GROUPS == 2 && (x / 32) % 2 != g) continue;
         uint32_t v[32];
         if (n > 0) {
-          tmem_ld32(from + x, v);
+          tmem_ld32(acc + x, v);
           tmem_wait_ld();
         } else {
 #pragma unroll

@@ -44,23 +44,52 @@ struct Tile {
 // stays empty, and the host needs no lengths.  Two more "clouds" cover the tokens
 // before the first and after the last offset; nobody attends there.
 inline int64_t packed_slots(int64_t tokens, int64_t clouds, int BM) { return tokens / BM + clouds + 2; }
+// The grid: heads within slots, so that the slots' order is the blocks' order.
+inline int packed_grid(int64_t tokens, int64_t clouds, int BM, int64_t heads, unsigned* blocks) {
+  const int64_t n = packed_slots(tokens, clouds, BM) * heads;
+  if (n >= (int64_t(1) << 31)) return set_error(TPO_ERR_UNSUPPORTED, "packed_attention: too many tokens times heads");
+  *blocks = (unsigned)n;
+  return TPO_OK;
+}
 
-// All 32 lanes of a warp call this with the same slot.  With at most 30 clouds every
-// lane holds one start and one round of loads does; else 32 probes a round narrow the range.
+// All 32 lanes of a warp call this with the same slot.
+//
+// With at most 30 clouds every lane holds one of them after one round of loads, and the
+// slots go to the clouds by falling length, so that no long tile starts last (late_first:
+// a cloud's last tile first, where causal rows see most keys).  With more, a search with
+// 32 probes a round finds the cloud, in the clouds' own order.
 __device__ __forceinline__ Tile find_tile(const int64_t* off, int64_t T, const int64_t* other,
-                                          int64_t To, int B, int BM, int64_t slot) {
+                                          int64_t To, int B, int BM, int64_t slot, int64_t slots,
+                                          bool late_first) {
   const int lane = threadIdx.x & 31;
+  if (slot == 0) {  // the first block of a head looks all offsets over
+    for (int i = lane; i < B; i += 32) {
+      const int64_t r0 = off[i], r1 = off[i + 1], o0 = other[i], o1 = other[i + 1];
+      if (r0 < 0 || r1 < r0 || r1 > T || o0 < 0 || o1 < o0 || o1 > To) atomicOr(&g_attention_error, kErrBadOffsets);
+    }
+  }
   // clamped start of extended cloud i in [0, B + 2], from its raw offset
   auto start = [&](int i, int64_t raw) -> int64_t { return i == 0 ? 0 : i >= B + 2 ? T : min64(max64(raw, 0), T); };
   int lo = 0, lo0 = 0;  // lane k holds the offsets of cloud lo0 + k
-  int64_t raw = 0, raw_other = 0;
+  int64_t raw = 0, raw_other = 0, tile;
   if (B + 2 <= 31) {
     const bool in = lane >= 1 && lane <= B + 1;
     raw = in ? off[lane - 1] : 0;
     raw_other = in ? other[lane - 1] : 0;
-    const unsigned m = __ballot_sync(0xffffffffu, lane < B + 2 && (lane == 0 || start(lane, raw) / BM + lane <= slot));
-    lo = 31 - __clz(m);
+    const int64_t s = start(lane, raw), e = __shfl_down_sync(0xffffffffu, s, 1);
+    const int len = lane < B + 2 ? (int)max64(e - s, 0) : 0;  // tokens fit 31 bits
+    int before = 0;  // tiles of longer clouds
+    for (int i = 0; i < B + 2; ++i) {
+      const int l = __shfl_sync(0xffffffffu, len, i);
+      if (l > len || (l == len && i < lane)) before += (l + BM - 1) / BM;
+    }
+    const int mine = (len + BM - 1) / BM;
+    const unsigned m = __ballot_sync(0xffffffffu, slot >= before && slot < before + mine);
+    lo = m ? __ffs(m) - 1 : 0;
+    tile = m ? slot - __shfl_sync(0xffffffffu, before, lo) : T;  // no tile left: behind every row
+    if (late_first && m) tile = __shfl_sync(0xffffffffu, mine, lo) - 1 - tile;
   } else {
+    if (late_first) slot = slots - 1 - slot;
     int hi = B + 2;
     while (hi - lo > 1) {  // greatest i in [lo, hi) with start(i)/BM + i <= slot
       const int width = (hi - lo + 31) / 32;
@@ -76,6 +105,7 @@ __device__ __forceinline__ Tile find_tile(const int64_t* off, int64_t T, const i
     const bool in = lane < 2 && i >= 1 && i <= B + 1;
     raw = in ? off[i - 1] : 0;
     raw_other = in ? other[i - 1] : 0;
+    tile = slot - (start(lo, __shfl_sync(0xffffffffu, raw, 0)) / BM + lo);
   }
   const int64_t r0 = __shfl_sync(0xffffffffu, raw, lo - lo0), r1 = __shfl_sync(0xffffffffu, raw, lo - lo0 + 1);
   const int64_t o0 = __shfl_sync(0xffffffffu, raw_other, lo - lo0), o1 = __shfl_sync(0xffffffffu, raw_other, lo - lo0 + 1);
@@ -83,7 +113,7 @@ __device__ __forceinline__ Tile find_tile(const int64_t* off, int64_t T, const i
   t.a0 = start(lo, r0);
   const int64_t end = start(lo + 1, r1);
   t.na = max64(end - t.a0, 0);
-  t.row0 = t.a0 + (slot - (t.a0 / BM + lo)) * BM;
+  t.row0 = t.a0 + tile * BM;
   t.rows = (int)max64(0, min64(end - t.row0, BM));
   if (t.row0 < t.a0) t.rows = 0;
   t.b0 = 0;
@@ -91,8 +121,6 @@ __device__ __forceinline__ Tile find_tile(const int64_t* off, int64_t T, const i
   if (lo >= 1 && lo <= B) {
     t.b0 = min64(max64(o0, 0), To);
     t.nb = max64(min64(max64(o1, 0), To) - t.b0, 0);
-    if (lane == 0 && (o0 < 0 || o1 < o0 || o1 > To || r0 < 0 || r1 < r0 || r1 > T))
-      atomicOr(&g_attention_error, kErrBadOffsets);
   }
   return t;
 }

@@ -150,9 +150,8 @@ __global__ void __launch_bounds__(Fwd<DP>::threads, Fwd<DP>::TILES == 2 ? 1 : 2)
   volatile int* abort = reinterpret_cast<volatile int*>(smem_raw + (s_abort - raw));
   unsigned* err = &g_attention_error;
 
-  const int warp = threadIdx.x / 32, head = blockIdx.y, kvh = head / (a.H / a.Hk);
-  const int64_t slot = a.causal ? (int64_t)gridDim.x - 1 - blockIdx.x : blockIdx.x;
-  const Tile t = find_tile(a.off_q, a.Tq, a.off_k, a.Tk, a.B, TILES * kTile, slot);
+  const int warp = threadIdx.x / 32, head = blockIdx.x % a.H, kvh = head / (a.H / a.Hk);
+  const Tile t = find_tile(a.off_q, a.Tq, a.off_k, a.Tk, a.B, TILES * kTile, blockIdx.x / a.H, gridDim.x / a.H, a.causal);
   if (t.rows <= 0) return;
   const int64_t shift = t.nb - t.na, first = t.row0 - t.a0;
   int steps[TILES], n = 0;  // key tiles that each query tile meets
@@ -433,9 +432,9 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
   unsigned* err = &g_attention_error;
 
   const int warp = threadIdx.x / 32, group = a.H / a.Hk;
-  const int64_t slot = !DKV && a.causal ? (int64_t)gridDim.x - 1 - blockIdx.x : blockIdx.x;
-  const Tile t = DKV ? find_tile(a.off_k, a.Tk, a.off_q, a.Tq, a.B, kTile, slot)
-                     : find_tile(a.off_q, a.Tq, a.off_k, a.Tk, a.B, kTile, slot);
+  const int heads = DKV ? a.Hk : a.H, slot = blockIdx.x / heads, slots = gridDim.x / heads;
+  const Tile t = DKV ? find_tile(a.off_k, a.Tk, a.off_q, a.Tq, a.B, kTile, slot, slots, false)
+                     : find_tile(a.off_q, a.Tq, a.off_k, a.Tk, a.B, kTile, slot, slots, a.causal);
   if (t.rows <= 0) return;
   const int64_t nq = DKV ? t.nb : t.na, nkeys = DKV ? t.na : t.nb, shift = nkeys - nq, first = t.row0 - t.a0;
   int64_t c_begin = 0, c_end = t.nb;  // columns that any row of the tile meets
@@ -444,8 +443,9 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
     else c_end = min64(c_end, max64(first + t.rows + shift, 0));
   }
   const int per_head = (int)max64(0, (c_end - c_begin + kCols - 1) / kCols);
-  const int kvh = DKV ? blockIdx.y : blockIdx.y / group;
-  const int head0 = DKV ? kvh * group : blockIdx.y;
+  const int block_head = blockIdx.x % heads;
+  const int kvh = DKV ? block_head : block_head / group;
+  const int head0 = DKV ? kvh * group : block_head;
   const int n = per_head * (DKV ? group : 1);
 
   if (warp == kMmaWarp) {
@@ -742,7 +742,9 @@ int fwd(const PackedArgs& a, cudaStream_t st) {
   auto kern = packed_mma_fwd_kernel<T, DP>;
   int s = set_smem(kern, F::smem);
   if (s) return s;
-  kern<<<dim3((unsigned)packed_slots(a.Tq, a.B, F::TILES * kTile), a.H), F::threads, F::smem, st>>>(a);
+  unsigned blocks;
+  if ((s = packed_grid(a.Tq, a.B, F::TILES * kTile, a.H, &blocks))) return s;
+  kern<<<blocks, F::threads, F::smem, st>>>(a);
   return check_launch();
 }
 
@@ -753,14 +755,18 @@ int bwd(const PackedArgs& a, cudaStream_t st) {
     auto kern = packed_mma_bwd_kernel<T, DP, true>;
     int s = set_smem(kern, W::smem);
     if (s) return s;
-    kern<<<dim3((unsigned)packed_slots(a.Tk, a.B, kTile), a.Hk), W::threads, W::smem, st>>>(a);
+    unsigned blocks;
+    if ((s = packed_grid(a.Tk, a.B, kTile, a.Hk, &blocks))) return s;
+    kern<<<blocks, W::threads, W::smem, st>>>(a);
     if ((s = check_launch())) return s;
   }
   if (a.dq && a.Tq > 0) {
     auto kern = packed_mma_bwd_kernel<T, DP, false>;
     int s = set_smem(kern, W::smem);
     if (s) return s;
-    kern<<<dim3((unsigned)packed_slots(a.Tq, a.B, kTile), a.H), W::threads, W::smem, st>>>(a);
+    unsigned blocks;
+    if ((s = packed_grid(a.Tq, a.B, kTile, a.H, &blocks))) return s;
+    kern<<<blocks, W::threads, W::smem, st>>>(a);
     if ((s = check_launch())) return s;
   }
   return TPO_OK;

@@ -191,10 +191,8 @@ __global__ void __launch_bounds__(kThreads) packed_simt_fwd_kernel(const PackedA
   float* vs = ks + BN * (DP + 4);
   float* ps = vs + BN * (DP + 4);
   const int tx = threadIdx.x % TX, ty = threadIdx.x / TX;
-  const int head = blockIdx.y, kvh = head / (a.H / a.Hk);
-  // causal rows late in a cloud see most keys: those blocks start first
-  const int64_t slot = a.causal ? (int64_t)gridDim.x - 1 - blockIdx.x : blockIdx.x;
-  const Tile t = find_tile(a.off_q, a.Tq, a.off_k, a.Tk, a.B, BM, slot);
+  const int head = blockIdx.x % a.H, kvh = head / (a.H / a.Hk);
+  const Tile t = find_tile(a.off_q, a.Tq, a.off_k, a.Tk, a.B, BM, blockIdx.x / a.H, gridDim.x / a.H, a.causal);
   if (t.rows <= 0) return;
   const int64_t shift = t.nb - t.na;            // a row sees keys up to its place + shift
   const int64_t first = t.row0 - t.a0;          // place of the tile's first row in its cloud
@@ -309,9 +307,9 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const int tx = lane % 8 + 8 * (warp % 2), ty = lane / 8 + 4 * (warp / 2);
   const int group = a.H / a.Hk;
-  const int64_t slot = !DKV && a.causal ? (int64_t)gridDim.x - 1 - blockIdx.x : blockIdx.x;
-  const Tile t = DKV ? find_tile(a.off_k, a.Tk, a.off_q, a.Tq, a.B, BM, slot)
-                     : find_tile(a.off_q, a.Tq, a.off_k, a.Tk, a.B, BM, slot);
+  const int nheads = DKV ? a.Hk : a.H, slot = blockIdx.x / nheads, slots = gridDim.x / nheads;
+  const Tile t = DKV ? find_tile(a.off_k, a.Tk, a.off_q, a.Tq, a.B, BM, slot, slots, false)
+                     : find_tile(a.off_q, a.Tq, a.off_k, a.Tk, a.B, BM, slot, slots, a.causal);
   if (t.rows <= 0) return;
   const int64_t nq = DKV ? t.nb : t.na, nkeys = DKV ? t.na : t.nb, shift = nkeys - nq;
   const int64_t first = t.row0 - t.a0;
@@ -322,8 +320,8 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
     else c_end = min64(c_end, max64(first + t.rows + shift, 0));
   }
   const float qscale = a.scale * kLog2e;
-  const int kvh = DKV ? blockIdx.y : blockIdx.y / group;
-  const int head0 = DKV ? kvh * group : blockIdx.y, heads = DKV ? group : 1;
+  const int block_head = blockIdx.x % nheads, kvh = DKV ? block_head : block_head / group;
+  const int head0 = DKV ? kvh * group : block_head, heads = DKV ? group : 1;
   const T* kp = (const T*)a.k + kvh * a.k_sh;
   const T* vp = (const T*)a.v + kvh * a.v_sh;
   float acc1[RM][DP / TX], acc2[DKV ? RM : 1][DKV ? DP / TX : 1];
@@ -471,7 +469,9 @@ int fwd(const PackedArgs& a, cudaStream_t st) {
   auto kern = packed_simt_fwd_kernel<T, VEC, DP, RM>;
   int s = set_smem(kern, Sh::smem);
   if (s) return s;
-  kern<<<dim3((unsigned)packed_slots(a.Tq, a.B, Sh::BM), a.H), kThreads, Sh::smem, st>>>(a);
+  unsigned blocks;
+  if ((s = packed_grid(a.Tq, a.B, Sh::BM, a.H, &blocks))) return s;
+  kern<<<blocks, kThreads, Sh::smem, st>>>(a);
   return check_launch();
 }
 
@@ -482,14 +482,18 @@ int bwd(const PackedArgs& a, cudaStream_t st) {
     auto kern = packed_simt_bwd_kernel<T, VEC, DP, RM, true>;
     int s = set_smem(kern, Sh::smem);
     if (s) return s;
-    kern<<<dim3((unsigned)packed_slots(a.Tk, a.B, Sh::BM), a.Hk), kThreads, Sh::smem, st>>>(a);
+    unsigned blocks;
+    if ((s = packed_grid(a.Tk, a.B, Sh::BM, a.Hk, &blocks))) return s;
+    kern<<<blocks, kThreads, Sh::smem, st>>>(a);
     if ((s = check_launch())) return s;
   }
   if (a.dq && a.Tq > 0) {
     auto kern = packed_simt_bwd_kernel<T, VEC, DP, RM, false>;
     int s = set_smem(kern, Sh::smem);
     if (s) return s;
-    kern<<<dim3((unsigned)packed_slots(a.Tq, a.B, Sh::BM), a.H), kThreads, Sh::smem, st>>>(a);
+    unsigned blocks;
+    if ((s = packed_grid(a.Tq, a.B, Sh::BM, a.H, &blocks))) return s;
+    kern<<<blocks, kThreads, Sh::smem, st>>>(a);
     if ((s = check_launch())) return s;
   }
   return TPO_OK;

@@ -31,11 +31,13 @@ struct PackedArgs {
 
 // A tile of one cloud: rows [row0, row0 + rows) of the packed tensor that was
 // tiled; [a0, a0 + na) and [b0, b0 + nb) are the cloud's rows there and in the
-// other tensor.  rows == 0: nothing to do.
+// other tensor.  rows == 0: nothing to do.  Tokens fit 31 bits (the host checks), and these
+// live in every warp of a block: 32-bit fields save it registers.
 struct Tile {
-  int64_t row0, a0, b0;
-  int rows;
-  int64_t na, nb;
+  int row0, rows, a0, na, b0, nb;
+  // Causal: a row at place x of the tiled side (from the cloud's start) sees keys below
+  // edge(x) + 1, or is seen by queries from edge(x) on.  Fits 32 bits in this order.
+  __device__ __forceinline__ int edge(int x) const { return (x - na) + nb; }
 };
 
 // Blocks per head for tiles of BM rows: with e(i) the start of cloud i, cloud i
@@ -62,12 +64,6 @@ __device__ __forceinline__ Tile find_tile(const int64_t* off, int64_t T, const i
                                           int64_t To, int B, int BM, int64_t slot, int64_t slots,
                                           bool late_first) {
   const int lane = threadIdx.x & 31;
-  if (slot == 0) {  // the first block of a head looks all offsets over
-    for (int i = lane; i < B; i += 32) {
-      const int64_t r0 = off[i], r1 = off[i + 1], o0 = other[i], o1 = other[i + 1];
-      if (r0 < 0 || r1 < r0 || r1 > T || o0 < 0 || o1 < o0 || o1 > To) atomicOr(&g_attention_error, kErrBadOffsets);
-    }
-  }
   // clamped start of extended cloud i in [0, B + 2], from its raw offset
   auto start = [&](int i, int64_t raw) -> int64_t { return i == 0 ? 0 : i >= B + 2 ? T : min64(max64(raw, 0), T); };
   int lo = 0, lo0 = 0;  // lane k holds the offsets of cloud lo0 + k
@@ -77,6 +73,9 @@ __device__ __forceinline__ Tile find_tile(const int64_t* off, int64_t T, const i
     raw = in ? off[lane - 1] : 0;
     raw_other = in ? other[lane - 1] : 0;
     const int64_t s = start(lane, raw), e = __shfl_down_sync(0xffffffffu, s, 1);
+    const int64_t next = __shfl_down_sync(0xffffffffu, raw, 1), next_other = __shfl_down_sync(0xffffffffu, raw_other, 1);
+    if (lane >= 1 && lane <= B && (raw < 0 || next < raw || next > T || raw_other < 0 || next_other < raw_other || next_other > To))
+      atomicOr(&g_attention_error, kErrBadOffsets);
     const int len = lane < B + 2 ? (int)max64(e - s, 0) : 0;  // tokens fit 31 bits
     int before = 0;  // tiles of longer clouds
     for (int i = 0; i < B + 2; ++i) {
@@ -89,6 +88,12 @@ __device__ __forceinline__ Tile find_tile(const int64_t* off, int64_t T, const i
     tile = m ? slot - __shfl_sync(0xffffffffu, before, lo) : T;  // no tile left: behind every row
     if (late_first && m) tile = __shfl_sync(0xffffffffu, mine, lo) - 1 - tile;
   } else {
+    if (slot == 0) {  // the first block of a head looks all offsets over
+      for (int i = lane; i < B; i += 32) {
+        const int64_t r0 = off[i], r1 = off[i + 1], o0 = other[i], o1 = other[i + 1];
+        if (r0 < 0 || r1 < r0 || r1 > T || o0 < 0 || o1 < o0 || o1 > To) atomicOr(&g_attention_error, kErrBadOffsets);
+      }
+    }
     if (late_first) slot = slots - 1 - slot;
     int hi = B + 2;
     while (hi - lo > 1) {  // greatest i in [lo, hi) with start(i)/BM + i <= slot
@@ -109,18 +114,17 @@ __device__ __forceinline__ Tile find_tile(const int64_t* off, int64_t T, const i
   }
   const int64_t r0 = __shfl_sync(0xffffffffu, raw, lo - lo0), r1 = __shfl_sync(0xffffffffu, raw, lo - lo0 + 1);
   const int64_t o0 = __shfl_sync(0xffffffffu, raw_other, lo - lo0), o1 = __shfl_sync(0xffffffffu, raw_other, lo - lo0 + 1);
+  const int64_t a0 = start(lo, r0), end = start(lo + 1, r1), row0 = a0 + tile * BM;
   Tile t;
-  t.a0 = start(lo, r0);
-  const int64_t end = start(lo + 1, r1);
-  t.na = max64(end - t.a0, 0);
-  t.row0 = t.a0 + tile * BM;
-  t.rows = (int)max64(0, min64(end - t.row0, BM));
-  if (t.row0 < t.a0) t.rows = 0;
-  t.b0 = 0;
-  t.nb = 0;
+  t.a0 = (int)a0;
+  t.na = (int)max64(end - a0, 0);
+  t.rows = row0 < a0 ? 0 : (int)max64(0, min64(end - row0, BM));
+  t.row0 = t.rows ? (int)row0 : 0;
+  t.b0 = t.nb = 0;
   if (lo >= 1 && lo <= B) {
-    t.b0 = min64(max64(o0, 0), To);
-    t.nb = max64(min64(max64(o1, 0), To) - t.b0, 0);
+    const int64_t b0 = min64(max64(o0, 0), To);
+    t.b0 = (int)b0;
+    t.nb = (int)max64(min64(max64(o1, 0), To) - b0, 0);
   }
   return t;
 }

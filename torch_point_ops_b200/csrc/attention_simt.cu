@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
   for (int r = 0; r < RM; ++r) {
     const int row = ty + TY * r;
     if (row >= t.rows) continue;
-    const int64_t at = DKV ? ((t.row0 + row) * a.Hk + kvh) * a.D : ((t.row0 + row) * a.H + head0) * a.D;
+    const int64_t at = ((int64_t)(t.row0 + row) * (DKV ? a.Hk : a.H) + (DKV ? kvh : head0)) * a.D;
     T* d1 = (T*)(DKV ? a.dk : a.dq) + at;
     T* d2 = DKV ? (T*)a.dv + at : nullptr;
 #pragma unroll

@@ -465,7 +465,7 @@ static int check_packed(const tpo_packed_attention* p) {
   if (!p) return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention: null problem");
   if (!attention_dtype(p->dtype)) return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention: dtype must be f32, f16 or bf16");
   if (p->clouds < 0 || p->clouds > (1 << 24) || p->tokens_q < 0 || p->tokens_k < 0 ||
-      p->tokens_q >= (int64_t(1) << 31) || p->tokens_k >= (int64_t(1) << 31))
+      p->tokens_q > INT32_MAX - 1024 || p->tokens_k > INT32_MAX - 1024)
     return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention: bad shape");
   if (p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads != 0 || p->heads > 65535)
     return fail(TPO_ERR_INVALID_ARGUMENT, "packed_attention: heads must be a multiple of kv_heads (at most 65535)");

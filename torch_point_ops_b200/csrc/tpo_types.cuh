@@ -45,6 +45,19 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
   return r;
 }
 
+// x and y as the sum of two rounded pairs: returns the first, `rest` gets what it left.
+template <typename T>
+__device__ __forceinline__ uint32_t split2(float x, float y, uint32_t& rest) {
+  const uint32_t first = pack2<T>(x, y);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    rest = pack2<T>(x - __uint_as_float(first << 16), y - __uint_as_float(first & 0xffff0000u));
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&first));
+    rest = pack2<T>(x - f.x, y - f.y);
+  }
+  return first;
+}
+
 // N elements (a power of two) that move as one access, or several of 16 bytes.
 template <typename T, int N>
 struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack { T v[N]; };

@@ -1,5 +1,6 @@
 /*
- * tpo_b200 -- C ABI of the B200-native chamfer / knn nearest-neighbour path.
+ * tpo_b200 -- C ABI of the B200-native chamfer / knn nearest-neighbour path, furthest
+ * point sampling, and the token operators (layer norm, attention).
  *
  * Plain pointers and sizes only; no torch types.  Every pointer argument is a
  * DEVICE pointer on the current CUDA device unless stated otherwise, all point
@@ -280,7 +281,8 @@ TPO_API int tpo_layer_norm_bwd(int dtype, int wdtype, const void* x, int64_t x_s
  * that cloud's tokens alone, whatever its neighbours hold.
  * dtype: TPO_F32, TPO_F16, TPO_BF16; width 1 to 256.  Strides are in elements, the
  * width dimension has stride 1.  Sums are fp32; for 16-bit types the probabilities
- * are rounded to that type before they multiply v (and dS before k and q). */
+ * are rounded to that type before they multiply v (and grad_o), and dS multiplies k
+ * and q as the sum of two values of that type. */
 typedef struct tpo_packed_attention {
   int dtype, causal;
   int64_t clouds, heads, kv_heads, width, tokens_q, tokens_k;

@@ -281,8 +281,8 @@ TPO_API int tpo_layer_norm_bwd(int dtype, int wdtype, const void* x, int64_t x_s
  * that cloud's tokens alone, whatever its neighbours hold.
  * dtype: TPO_F32, TPO_F16, TPO_BF16; width 1 to 256.  Strides are in elements, the
  * width dimension has stride 1.  Sums are fp32; for 16-bit types the probabilities
- * are rounded to that type before they multiply v (and grad_o), and dS multiplies k
- * and q as the sum of two values of that type. */
+ * are rounded to that type before they multiply v (and grad_o), as is dS before it
+ * multiplies q; dS multiplies k as the sum of two values of that type. */
 typedef struct tpo_packed_attention {
   int dtype, causal;
   int64_t clouds, heads, kv_heads, width, tokens_q, tokens_k;
@@ -296,7 +296,8 @@ typedef struct tpo_packed_attention {
 TPO_API int tpo_packed_attention_fwd(const tpo_packed_attention* p, void* o, float* lse, void* stream);
 /* dq (tokens_q, heads, width), dk, dv (tokens_k, kv_heads, width), contiguous, fully
  * written, each NULL where it is not wanted (dk and dv together).  No atomics touch
- * them: every run gives the same bits. */
+ * them: every run gives the same bits, whichever are asked for (on the tensor cores
+ * dk and dv need what dq's kernel sums, so that kernel runs for them too). */
 TPO_API size_t tpo_packed_attention_bwd_workspace_size(int64_t tokens_q, int64_t heads);
 TPO_API int tpo_packed_attention_bwd(const tpo_packed_attention* p, const void* o, const float* lse,
                                      const void* grad_o, int64_t grad_o_token_stride,

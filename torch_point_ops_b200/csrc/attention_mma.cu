@@ -7,10 +7,12 @@
 //
 // The tensor cores take no wider operand beside 16-bit ones.  P is rounded to 16 bits
 // before it multiplies V (and dO): that adds about as much error as the rounding of the
-// result.  dS, a difference of large terms that the gradients sum up, travels as two
-// 16-bit values (its rounding and what that left): with one, dQ and dK of causal clouds are
-// 1.5 to 1.6 times as far from the exact ones as their own rounding puts them, with two 1.1
-// times, for a tenth of the backward's time.  Every sum, maximum, P and dS themselves are fp32.
+// result.  dS is a difference of large terms that the gradients sum up.  With delta from
+// the rounded O and one rounding, dQ and dK of causal clouds come out 1.5 to 1.6 times as
+// far from the exact ones as their own rounding puts them.  So for dQ it travels as two 16-bit
+// values (its rounding and what that left: 1.1 times); the dQ kernel also sums delta = P dP
+// without O's rounding, and with that one rounding does for dK (1.4 times).
+// Every sum, maximum, P and dS themselves are fp32.
 #include <type_traits>
 
 #include "attention_common.cuh"
@@ -558,15 +560,15 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
           if (DKV) {
             bar_wait(b_p + 8 * g, parity, abort, err);
             tc_fence_after();
-            fence_async_smem();  // the copies landed before S was computed
+            ring.wait_operand(2 * j + 1);
             mma_nn<T, DP, kCols>(one, u_tmem + W::acc2, s_of(j), y_of(2 * j + 1), j > 0);
             if (j + GROUPS < un) mma_commit(one, b_used2 + 8 * g);
           }
           bar_wait(b_ds + 8 * g, parity, abort, err);
           tc_fence_after();
-          fence_async_smem();
+          fence_async_smem();  // y1 has landed: the other warp waited for it before S, and dS came after S
           mma_nn<T, DP, kCols>(one, u_tmem + W::acc1, s_of(j) + 64, y_of(2 * j), j > 0);
-          mma_nn<T, DP, kCols>(one, u_tmem + W::acc1, s_of(j) + 96, y_of(2 * j), true);
+          if (!DKV) mma_nn<T, DP, kCols>(one, u_tmem + W::acc1, s_of(j) + 96, y_of(2 * j), true);
           if (j + GROUPS < un) mma_commit(one, b_used1 + 8 * g);
           ring.release(one, 2 * j);
           if (DKV) ring.release(one, 2 * j + 1);  // not before: the threads read delta from it
@@ -600,6 +602,7 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
       row_lse = a.lse2[(int64_t)head0 * a.Tq + t.row0 + row];
       row_delta = a.delta[(int64_t)head0 * a.Tq + t.row0 + row];
     }
+    u64 exact[2] = {0, 0};  // this row's sum of P dP over the group's tiles: delta without O's rounding (not DKV)
     // one step's row: P from S, then dS from dP
     auto step_rows = [&](int j, int lo, int hi, auto masked) {
       constexpr bool MASK = decltype(masked)::value;
@@ -675,6 +678,10 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
             d0 = d1 = pk(row_delta, row_delta);
           }
           const uint32_t* s = &v[h][2 * k];
+          if (!DKV) {
+            exact[0] = fma2(p[i], pku(s[0], s[1]), exact[0]);
+            exact[1] = fma2(p[i + 1], pku(s[2], s[3]), exact[1]);
+          }
           u64 a0 = mul2(p[i], sub2(pku(s[0], s[1]), d0)), a1 = mul2(p[i + 1], sub2(pku(s[2], s[3]), d1));
           if (std::is_same<T, __half>::value) a0 = mul2(a0, pk(c, c)), a1 = mul2(a1, pk(c, c));
           float x[4];
@@ -684,11 +691,16 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = 2 * i + e >= lo && 2 * i + e < hi ? x[e] : 0.f;
           }
-          hi16[k] = split2<T>(x[0], x[1], lo16[k]);
-          hi16[k + 1] = split2<T>(x[2], x[3], lo16[k + 1]);
+          if (DKV) {
+            hi16[k] = pack2<T>(x[0], x[1]);
+            hi16[k + 1] = pack2<T>(x[2], x[3]);
+          } else {
+            hi16[k] = split2<T>(x[0], x[1], lo16[k]);
+            hi16[k + 1] = split2<T>(x[2], x[3], lo16[k + 1]);
+          }
         }
         tmem_st16(tdp + 16 * h, hi16);
-        tmem_st16(tdp + 32 + 16 * h, lo16);
+        if (!DKV) tmem_st16(tdp + 32 + 16 * h, lo16);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -706,6 +718,18 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
       for (step += GROUPS; step >= per_head;) step -= per_head;
       if (__all_sync(0xffffffffu, lo == 0 && hi == kCols)) step_rows(j, lo, hi, std::false_type{});
       else step_rows(j, lo, hi, std::true_type{});
+    }
+    if (!DKV && n > 0) {  // for the kernel of dK and dV, which runs next
+      float x, y;
+      upk(add2(exact[0], exact[1]), x, y);
+      x += y;
+      if (GROUPS == 2) {
+        float* other = const_cast<float*>(stats);  // no statistics travel with keys: the space is free
+        if (g == 1) other[row] = x;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (g == 0) x += other[row];
+      }
+      if (g == 0 && live) a.delta[(int64_t)head0 * a.Tq + t.row0 + row] = x;
     }
     if (n > 0) {
       bar_wait(b_done, 0, abort, err);
@@ -730,7 +754,7 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = 0;
         }
-        if (live) store32<T>(op, v, f, x, a.D);
+        if (live && (DKV || a.dq)) store32<T>(op, v, f, x, a.D);
       }
     }
     tc_fence_before();
@@ -762,21 +786,22 @@ int fwd(const PackedArgs& a, cudaStream_t st) {
 template <typename T, int DP>
 int bwd(const PackedArgs& a, cudaStream_t st) {
   using W = Bwd<DP>;
+  // dQ first, wanted or not: it leaves an exact delta
+  if ((a.dq || a.dk) && a.Tq > 0) {
+    auto kern = packed_mma_bwd_kernel<T, DP, false>;
+    int s = set_smem(kern, W::smem);
+    if (s) return s;
+    unsigned blocks;
+    if ((s = packed_grid(a.Tq, a.B, kTile, a.H, &blocks))) return s;
+    kern<<<blocks, W::threads, W::smem, st>>>(a);
+    if ((s = check_launch())) return s;
+  }
   if (a.dk && a.Tk > 0) {
     auto kern = packed_mma_bwd_kernel<T, DP, true>;
     int s = set_smem(kern, W::smem);
     if (s) return s;
     unsigned blocks;
     if ((s = packed_grid(a.Tk, a.B, kTile, a.Hk, &blocks))) return s;
-    kern<<<blocks, W::threads, W::smem, st>>>(a);
-    if ((s = check_launch())) return s;
-  }
-  if (a.dq && a.Tq > 0) {
-    auto kern = packed_mma_bwd_kernel<T, DP, false>;
-    int s = set_smem(kern, W::smem);
-    if (s) return s;
-    unsigned blocks;
-    if ((s = packed_grid(a.Tq, a.B, kTile, a.H, &blocks))) return s;
     kern<<<blocks, W::threads, W::smem, st>>>(a);
     if ((s = check_launch())) return s;
   }

@@ -431,7 +431,8 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const PackedArgs a, i
     int64_t tok = 0;
     int head = 0;
     if (r < rows) {
-      tok = r / a.H;
+      // a 64-bit division costs more than the row itself
+      tok = rows <= 0xffffffffll ? (int64_t)((uint32_t)r / (uint32_t)a.H) : r / a.H;
       head = (int)(r - tok * a.H);
       const T* o = (const T*)a.o + r * a.D;
       const T* g = (const T*)a.go + tok * a.go_st + head * a.go_sh;

@@ -96,23 +96,36 @@ __global__ void __launch_bounds__(TPR* RPB)
   constexpr int NV = EPT / VEC;
   // 32 and 64 bits: the next row is on its way while this one is reduced and written.
   // 16 bits: conversions keep the issue slots busy, and the registers of a second
-  // row cost more warps than it brings (measured, 32768 x 1024: 30.7 against 29.7 us).
+  // row cost more warps than it brings (measured, 32768 x 1024: 26.6 against 25.8 us).
   constexpr bool AHEAD = sizeof(T) != 2;
   __shared__ A red[RPB][4][TPR / 32];
   const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
   const A eps = (A)eps_, inv_c = (A)1 / (A)C;
   const int64_t step = (int64_t)gridDim.x * RPB;
   int64_t row = (int64_t)blockIdx.x * RPB + g;
-  if (row >= rows) return;  // a whole row group: its barrier is its own
+  // Whole vectors of 16-bit rows: the parameters wait in shared memory, their registers
+  // would cost a third of the warps (measured, 32768 x 1024: 30.1 against 25.8 us).
+  constexpr bool SHARED = sizeof(T) == 2 && VEC == 8 && EPT > 8 && 2 * NV * TPR * sizeof(Pack<W, VEC>) <= 40960;
+  __shared__ Pack<W, VEC> ws[SHARED ? NV * TPR : 1], bs[SHARED ? NV * TPR : 1];
   Pack<T, VEC> cur[NV], nxt[NV];
   Pack<W, VEC> wv[NV], bv[NV];
   fill(cur, 0);
   fill(nxt, 0);
   fill(wv, 1);  // no weight, no bias: one and zero, so that the loop has no branches
   fill(bv, 0);
+  if (SHARED) {
+    if (g == 0) {
+      if (w) load_row<VEC, TPR, EPT>(wv, w, t, C);
+      if (b) load_row<VEC, TPR, EPT>(bv, b, t, C);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) ws[i * TPR + t] = wv[i], bs[i * TPR + t] = bv[i];
+    }
+    __syncthreads();
+  }
+  if (row >= rows) return;  // a whole row group: its barrier is its own
   load_row<VEC, TPR, EPT>(cur, x + row * xs, t, C);
-  if (w) load_row<VEC, TPR, EPT>(wv, w, t, C);
-  if (b) load_row<VEC, TPR, EPT>(bv, b, t, C);
+  if (!SHARED && w) load_row<VEC, TPR, EPT>(wv, w, t, C);
+  if (!SHARED && b) load_row<VEC, TPR, EPT>(bv, b, t, C);
   int phase = 0;
   while (row < rows) {
     const int64_t next = row + step;
@@ -142,8 +155,8 @@ __global__ void __launch_bounds__(TPR* RPB)
     for (int i = 0; i < NV; ++i) {
       const int c = (i * TPR + t) * VEC;
       A o[VEC], wk[VEC], bk[VEC];
-      unpack<VEC, 1>(wk, reinterpret_cast<const Pack<W, VEC>(&)[1]>(wv[i]));
-      unpack<VEC, 1>(bk, reinterpret_cast<const Pack<W, VEC>(&)[1]>(bv[i]));
+      unpack<VEC, 1>(wk, reinterpret_cast<const Pack<W, VEC>(&)[1]>(SHARED ? ws[i * TPR + t] : wv[i]));
+      unpack<VEC, 1>(bk, reinterpret_cast<const Pack<W, VEC>(&)[1]>(SHARED ? bs[i * TPR + t] : bv[i]));
 #pragma unroll
       for (int j = 0; j < VEC; ++j) o[j] = v[i * VEC + j] * rstd * wk[j] + bk[j];
       if (c < C) store_vec<VEC>(y + row * C + c, o);

@@ -13,6 +13,14 @@
 // values (its rounding and what that left: 1.1 times); the dQ kernel also sums delta = P dP
 // without O's rounding, and with that one rounding does for dK (1.4 times).
 // Every sum, maximum, P and dS themselves are fp32.
+//
+// Measured (B200, bf16, 4 causal clouds of 4096 tokens, 16 heads; of the products that the
+// formulas need): width 128 forward 270 to 280 us (1.0 PFLOP/s; two clouds without causal: 1.1),
+// dQ and dK dV together 1.24 ms (0.55); width 64 forward 240 to 275 us, backward 0.76 to
+// 0.81 ms.  Width 128: the tensor pipe is 47 to 49 % busy, P V and the next S follow one another
+// on the tile that waits for them.  Width 64: the exponentials (special-function unit 57 %
+// busy) and the row threads' issue slots.  The clock falls to 1.4 to 1.6 GHz under the power
+// limit in long runs.
 #include <type_traits>
 
 #include "attention_common.cuh"

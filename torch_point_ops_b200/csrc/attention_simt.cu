@@ -19,9 +19,13 @@
 // cycles and leave every other issue slot to loads.  Outputs are single FMAs: pairs would
 // need one operand doubled in registers, and the moves cost more than they save.  The
 // probabilities are kept transposed, a thread's rows side by side.  A warp is
-// 4 rows x 8 columns, so that both kinds of operand load are one shared-memory
-// wavefront (rows of DP + 4 floats: neighbouring rows lie in different banks): 12
-// wavefronts per 64 FMAs with 4 x 8 results per thread, 8 per 32 with 4 x 4.
+// 4 rows x 8 columns; rows of operand tiles have DP + 4 floats, so that neighbouring
+// rows lie in different banks.
+//
+// Measured (B200, fp32, 8 clouds of 2048 tokens, 16 heads of width 64): forward 3.63 ms, 38
+// TFLOP/s of the two products; dQ and dK dV 34 TFLOP/s.  The FP32 pipe is 50 to 56 % busy,
+// the shared-memory pipe 65 to 75 %: operand loads are the bound (larger results per
+// thread would need fewer of them, and more registers than there are).
 #include "attention_common.cuh"
 
 namespace tpo {

@@ -10,6 +10,11 @@
 // moments and the result; the variance is the centred second pass over those
 // registers, which loses nothing when |mean| >> std.  All sums are fp32 (fp64 for
 // fp64 rows); outputs are rounded once.
+//
+// Measured (B200, GB/s of the passes above; a plain copy moves 6555): forward 65536 x 512 fp32
+// 42.6 us (6300), 32768 x 1024 bf16 25.8 us (5210: issue slots, conversions), 10007 x 771
+// fp16 11.3 us (2720: one element per load); backward 67.7 us (5950), 39.3 us (5120),
+// 16.3 us (2840).
 #include "tpo_internal.h"
 #include "tpo_types.cuh"
 

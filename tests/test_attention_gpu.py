@@ -379,6 +379,20 @@ def test_cached_strides_and_lengths_out_of_range(dtype):
     _check_cached(q, wide[..., ::2], wide[..., 1::2], [90, 17])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (20, 1, 128), (6, 2, 200), (3, 3, 33)])
+@pytest.mark.parametrize("P", [32, 65, 127, 129, 255, 257, 513, 1024, 1025])
+def test_cached_short_axes(P, H, Hk, D, dtype):
+    # lengths that end in each part of the axis, leave parts empty, or all of it
+    lengths = [P, 1, 0, P // 2 + 1, P - 1, P // 8]
+    q, k, v = _cached_inputs(len(lengths), P, H, Hk, D, dtype)
+    for n, length in enumerate(lengths):
+        k[n, length:], v[n, length:] = math.nan, math.inf
+    want = _check_cached(q, k, v, lengths)
+    for _ in range(20):  # and the same bits each time
+        assert torch.equal(tpo.cached_attention(q, k, v, torch.tensor(lengths, device=DEV)), want)
+
+
 def test_cached_offsets_beyond_32_bits():
     # the last cloud's cache starts 2.2e9 elements into the tensor
     P, N = 70000, 250

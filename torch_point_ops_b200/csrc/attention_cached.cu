@@ -5,18 +5,19 @@
 //
 // Two to four operations per byte of cache: HBM is the bound, so every cached
 // token is read once for all query heads of its group.  The key axis is cut into chunks
-// of a fixed number of tokens
-// (chosen by the host from N, Hk and P, so no length is copied to the host); a
-// block takes one chunk of one (cloud, kv head), blocks beyond a cloud's length
-// leave at once, and with more than one chunk the unnormalised partials are
-// joined in chunk order by a second small kernel.
+// of a fixed number of tokens (chosen by the host from N, Hk and P, so no length is copied
+// to the host); a block takes one chunk of one (cloud, kv head).  Up to 8 short chunks are a
+// thread-block cluster, which joins them through its shared memory in chunk order.  More
+// or longer ones: blocks beyond a cloud's length leave at once, and the unnormalised
+// partials are joined in chunk order by a second small kernel.
 //
 // Slots at or beyond lengths[n] are never read: they may hold anything.
 //
 // Measured (B200, bf16, width 128): 64 clouds of 4096 tokens, 32 heads over 8: 180 us, 5.97
 // TB/s of cache; one cloud of 131072 tokens, 16 heads over 4: 50 us, 5.4 TB/s (a plain copy
 // moves 6.56); fp32, 8 ragged clouds of up to 16384 tokens: 60 us, 4.2 TB/s.  What is left is
-// the start of the blocks, the join (4 us) and, in fp32, load latency.
+// the start of the blocks, the join (4 us) and, in fp32, load latency.  One cloud of 256 tokens,
+// 8 heads of width 64: 4.8 us, a chain of latencies.
 #include "attention_common.cuh"
 #include "tcgen05.cuh"  // asynchronous copies
 
@@ -33,6 +34,7 @@ struct CachedArgs {
   float* part;  // (N*H, chunks, pitch) sums, then (N*H, chunks, 2) maxima (base 2) and weights
   int64_t P, chunk;
   int N, H, Hk, D, chunks;
+  int cluster;  // the chunks of a (cloud, kv head) are one thread-block cluster, which joins them itself
   float qscale;  // scale * log2(e)
 };
 
@@ -54,6 +56,47 @@ __device__ __forceinline__ void put(const CachedArgs& a, int64_t row, int chunk,
     a.part[(row * a.chunks + chunk) * part_pitch(a.D) + c] = sum;
 }
 
+// The chunks' sums of `rows` heads (res[row * pitch + c], {maximum, weight} in rs[row], in every
+// block's shared memory at the same place) joined by the cluster in chunk order; the
+// blocks share the columns.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ float remote(uint32_t addr, int rank) {
+  float v;
+  asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
+               : "=f"(v)
+               : "r"(addr), "r"(rank)
+               : "memory");
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void cluster_join(const CachedArgs& a, int chunk, int64_t row0, int rows, const float* res,
+                                             int pitch, const float2* rs) {
+  cluster_sync();
+  const uint32_t r = smem_addr(res), st = smem_addr(rs);
+  for (int i = chunk * kThreads + threadIdx.x; i < rows * a.D; i += a.chunks * kThreads) {
+    const int row = i / a.D, c = i - row * a.D;
+    float m[8], mx = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      m[k] = k < a.chunks ? remote(st + row * 8, k) : -INFINITY;
+      mx = fmaxf(mx, m[k]);
+    }
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float sum = 0.f, l = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k >= a.chunks) continue;
+      const float f = exp2f(m[k] - base);
+      sum = fmaf(f, remote(r + (row * pitch + c) * 4, k), sum);
+      l = fmaf(f, remote(st + row * 8 + 4, k), l);
+    }
+    ((T*)a.o)[(row0 + row) * a.D + c] = from_acc<T>(l > 0.f ? sum / l : l == 0.f ? 0.f : l);
+  }
+  cluster_sync();  // nobody leaves while its shared memory is read
+}
+
 // ---------------------------------------------------------------------------
 // Any dtype, any strides, D <= 256.  A warp takes 32 keys at a time: LPK lanes
 // share a key's row (NVL vectors of VEC elements each), so 32 / LPK keys are read
@@ -61,13 +104,15 @@ __device__ __forceinline__ void put(const CachedArgs& a, int64_t row, int chunk,
 // softmax; the values are read with the lanes laid out as for the keys.  GB query
 // heads of the group per block.
 // ---------------------------------------------------------------------------
-template <typename T, int VEC, int LPK, int NVL, int GB>
-__global__ void __launch_bounds__(kThreads) cached_simt_kernel(const CachedArgs a) {
+template <typename T, int VEC, int LPK, int NVL, int GB, bool CLUSTER>  // one kernel for both: 192 -> 260 us, by registers
+__global__ void __launch_bounds__(kThreads) cached_simt_kernel(CachedArgs a) {
   constexpr int UNR = GB <= 2 ? 8 : 4;
   constexpr int KPI = 32 / LPK, W = LPK * NVL * VEC;
   __shared__ float sc[kWarps][GB][32];
   __shared__ float jm[kWarps][GB], jl[kWarps][GB];
   __shared__ float jo[kWarps][GB][W];
+  __shared__ float res[CLUSTER ? GB * W : 1];
+  __shared__ float2 rs[CLUSTER ? GB : 1];
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   const int kl = lane % LPK, kr = lane / LPK;
   const int group = a.H / a.Hk, gblocks = (group + GB - 1) / GB;
@@ -75,7 +120,7 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const CachedArgs 
   const int gn = min(GB, group - g0);
   const int64_t len = length_of(a, n);
   const int64_t j_begin = (int64_t)chunk * a.chunk, j_end = min64(len, j_begin + a.chunk);
-  if (chunk > 0 && j_begin >= len) return;  // the join skips this chunk too
+  if (!CLUSTER && chunk > 0 && j_begin >= len) return;  // the join skips this chunk too
   const int64_t row0 = (int64_t)n * a.H + kvh * group + g0;
   float q[GB][NVL][VEC], acc[GB][NVL][VEC], m[GB], l[GB];
 #pragma unroll
@@ -190,6 +235,11 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const CachedArgs 
       sum += f * jo[w][g][c];
       ls += f * jl[w][g];
     }
+    if (CLUSTER) {
+      res[g * W + c] = sum;
+      if (c == 0) rs[g] = make_float2(mx, ls);
+      continue;
+    }
     put<T>(a, row0 + g, chunk, c, sum, ls);
     if (a.chunks > 1 && c == 0) {
       float* st = part_stats(a) + ((row0 + g) * a.chunks + chunk) * 2;
@@ -197,6 +247,7 @@ __global__ void __launch_bounds__(kThreads) cached_simt_kernel(const CachedArgs 
       st[1] = ls;
     }
   }
+  if (CLUSTER) cluster_join<T>(a, chunk, row0, gn, res, W, rs);
 }
 
 // ---------------------------------------------------------------------------
@@ -243,15 +294,16 @@ struct MmaShape {
   static constexpr int tile = 16 * (kp + vp);
   static constexpr int stages = DP == 128 ? 2 : 3;  // three blocks per SM: measured against two blocks with a longer queue
   static constexpr int smem = kWarps * stages * tile;  // also holds the join: 16 rows of DP + 4 floats per warp
-  static_assert(stages * tile >= 16 * (DP + 4) * 4, "join buffer");
+  static_assert(smem >= kWarps * 16 * (DP + 4) * 4 + 16 * DP * 4, "join buffers");
 };
 
-template <typename T, int DP, bool TALL>  // TALL: the block has more than 8 heads
-__global__ void __launch_bounds__(kThreads, 3) cached_mma_kernel(const CachedArgs a) {
+template <typename T, int DP, bool TALL, bool CLUSTER>  // TALL: the block has more than 8 heads
+__global__ void __launch_bounds__(kThreads, 3) cached_mma_kernel(CachedArgs a) {
   using Sh = MmaShape<DP>;
   constexpr int KC = Sh::KC, VC = Sh::VC, ST = Sh::stages;
   __shared__ float jm[kWarps][16], jl[kWarps][16];
   __shared__ unsigned long long full[kWarps][ST];
+  __shared__ float2 rs[16];
   extern __shared__ uint4 ring[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane / 4, c = lane % 4;
   const int group = a.H / a.Hk, gblocks = (group + 15) / 16;
@@ -259,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 3) cached_mma_kernel(const CachedArg
   const int gn = min(16, group - g0);
   const int64_t len = length_of(a, n);
   const int64_t j_begin = (int64_t)chunk * a.chunk, j_end = min64(len, j_begin + a.chunk);
-  if (chunk > 0 && j_begin >= len) return;  // the join skips this chunk too
+  if (!CLUSTER && chunk > 0 && j_begin >= len) return;  // the join skips this chunk too
   pdl_trigger();
   const T* kp = (const T*)a.k + n * a.k_sn + kvh * a.k_sh;
   const T* vp = (const T*)a.v + n * a.v_sn + kvh * a.v_sh;
@@ -399,6 +451,7 @@ __global__ void __launch_bounds__(kThreads, 3) cached_mma_kernel(const CachedArg
   // the warps' rows, joined in order (every copy has been waited for)
   __syncthreads();
   float* jo = reinterpret_cast<float*>(ring);  // [warp][row][DP + 4]
+  float* res = jo + kWarps * 16 * (DP + 4);    // [row][DP]
 #pragma unroll
   for (int r = 0; r < (TALL ? 2 : 1); ++r) {
     float x = l[r];
@@ -437,13 +490,21 @@ __global__ void __launch_bounds__(kThreads, 3) cached_mma_kernel(const CachedArg
       ls += f * jl[w][row];
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) put<T>(a, row0 + row, chunk, col + e, sum[e], ls);
+    for (int e = 0; e < 4; ++e) {
+      if (CLUSTER) res[row * DP + col + e] = sum[e];
+      else put<T>(a, row0 + row, chunk, col + e, sum[e], ls);
+    }
+    if (CLUSTER) {
+      if (col == 0) rs[row] = make_float2(mx, ls);
+      continue;
+    }
     if (a.chunks > 1 && col == 0) {
       float* st = part_stats(a) + ((row0 + row) * a.chunks + chunk) * 2;
       st[0] = mx;
       st[1] = ls;
     }
   }
+  if (CLUSTER) cluster_join<T>(a, chunk, row0, gn, res, DP, rs);
 }
 
 // Joins the chunks of a head's row: o = sum_c 2^(m_c - m) sum_c / sum_c 2^(m_c - m) l_c.
@@ -528,10 +589,23 @@ __global__ void __launch_bounds__(256) cached_join_kernel(const CachedArgs a) {
 // by its registers (for the common widths).
 constexpr int kMmaBlocks = 3, kSimtBlocks = 8;
 
-// Tokens per chunk.  One cloud: as many chunks as blocks fit on the GPU at once.  Several: two such waves and at least five chunks each, since their lengths
-// are not known here and differ.  Splitting a short axis costs a join (about 4 us): with enough
+// Chunks of a short axis that one cluster joins, with no second launch and no workspace: 8, 4 or
+// 2, of 33 to 128 tokens, while two blocks per SM hold them all; else 1.  Measured against
+// chunks and a join: 300 tokens, 8 heads of 64, bf16: 4.8 against 7.0 us; 1024 tokens: 6.4 and
+// 6.4 us, the whole call 8.2 against 9.8.  Longer chunks lose, since a cluster ends at 8:
+// 2048 tokens 9.1 against 6.6 us.
+int cluster_chunks(int64_t N, int64_t Hk, int64_t P) {
+  for (int c = 8; c > 1; c /= 2)
+    if (N * Hk * c <= 148 * 2 && P > 32 * c) return P <= 128 * c ? c : 1;
+  return 1;
+}
+
+// Tokens per chunk.  One cloud: as many chunks as blocks fit on the GPU at once.
+// Several: two such waves and at least five chunks each, since their lengths are not
+// known here and differ.  Splitting a short axis costs a join (about 4 us): with enough
 // blocks without it, not below 512 tokens.
 int64_t chunk_tokens(int64_t N, int64_t Hk, int64_t P, int per_sm) {
+  if (const int c = cluster_chunks(N, Hk, P); c > 1) return (P + c - 1) / c;
   const int64_t pairs = max64(1, N * Hk), waves = 148 * per_sm, least = pairs < 148 ? 64 : 512;
   const int64_t wish = N == 1 ? waves / pairs : max64(2 * waves / pairs, 5);
   const int64_t chunks = max64(1, min64((P + least - 1) / least, wish));
@@ -542,12 +616,32 @@ int64_t chunk_count(int64_t N, int64_t Hk, int64_t P, int per_sm) {
   return max64(1, (P + c - 1) / c);
 }
 
+int chunk_launch(void (*kern)(CachedArgs), dim3 grid, int smem, const CachedArgs& a, cudaStream_t st) {
+  if (!a.cluster) {
+    kern<<<grid, kThreads, smem, st>>>(a);
+    return check_launch();
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = 1;
+  at[0].val.clusterDim.y = a.chunks;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kern, a));
+}
+
 template <typename T, int VEC, int LPK, int NVL, int GB>
 int simt_launch(const CachedArgs& a, cudaStream_t st) {
   const int gblocks = (a.H / a.Hk + GB - 1) / GB;
-  cached_simt_kernel<T, VEC, LPK, NVL, GB>
-      <<<dim3(a.Hk * gblocks, a.chunks, a.N), kThreads, 0, st>>>(a);
-  return check_launch();
+  const auto kern =
+      a.cluster ? cached_simt_kernel<T, VEC, LPK, NVL, GB, true> : cached_simt_kernel<T, VEC, LPK, NVL, GB, false>;
+  return chunk_launch(kern, dim3(a.Hk * gblocks, a.chunks, a.N), 0, a, st);
 }
 template <typename T, int VEC, int LPK, int NVL>
 int simt_group(const CachedArgs& a, cudaStream_t st) {
@@ -578,12 +672,13 @@ template <typename T, int DP>
 int mma_launch(const CachedArgs& a, cudaStream_t st) {
   const int group = a.H / a.Hk;
   const dim3 grid(a.Hk * ((group + 15) / 16), a.chunks, a.N);  // neighbours read the same tokens' heads
-  auto kern = group > 8 ? cached_mma_kernel<T, DP, true> : cached_mma_kernel<T, DP, false>;
+  const auto kern = a.cluster ? group > 8 ? cached_mma_kernel<T, DP, true, true> : cached_mma_kernel<T, DP, false, true>
+                    : group > 8 ? cached_mma_kernel<T, DP, true, false>
+                                : cached_mma_kernel<T, DP, false, false>;
   constexpr int smem = MmaShape<DP>::smem;
   const int s = cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   if (s) return s;
-  kern<<<grid, kThreads, smem, st>>>(a);
-  return check_launch();
+  return chunk_launch(kern, grid, smem, a, st);
 }
 
 template <typename T>
@@ -592,12 +687,14 @@ int cached_typed(CachedArgs a, cudaStream_t st) {
   const bool mma = sizeof(T) == 2 && a.D <= 128 && aligned16<T>(a);
   const int per_sm = mma ? kMmaBlocks : kSimtBlocks;
   a.chunk = chunk_tokens(a.N, a.Hk, a.P, per_sm);
+  a.cluster = cluster_chunks(a.N, a.Hk, a.P) > 1;
   a.chunks = (int)chunk_count(a.N, a.Hk, a.P, per_sm);
+  const bool joined = a.cluster || a.chunks == 1;
   int s;
   if constexpr (sizeof(T) == 2) {
     if (mma) {
       s = a.D <= 64 ? mma_launch<T, 64>(a, st) : mma_launch<T, 128>(a, st);
-      if (s || a.chunks == 1) return s;
+      if (s || joined) return s;
       return join_launch<T>(a, st);
     }
   }
@@ -610,13 +707,14 @@ int cached_typed(CachedArgs a, cudaStream_t st) {
     else if (a.D <= 128) s = simt_group<T, 1, 32, 4>(a, st);
     else s = simt_group<T, 1, 32, 8>(a, st);
   }
-  if (s || a.chunks == 1) return s;
+  if (s || joined) return s;
   return join_launch<T>(a, st);
 }
 
 }  // namespace
 
 size_t cached_workspace_size(int64_t N, int64_t H, int64_t Hk, int64_t P, int64_t D) {
+  if (cluster_chunks(N, Hk, P) > 1) return 0;
   const int64_t chunks = max64(chunk_count(N, Hk, P, kMmaBlocks), chunk_count(N, Hk, P, kSimtBlocks));
   return chunks == 1 ? 0 : (size_t)(N * H) * chunks * (part_pitch((int)D) + 2) * sizeof(float);
 }

@@ -22,11 +22,11 @@ size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 }  // namespace
 
-// [delta][lse in base 2][largest |grad_o|], each (heads, tokens_q)
+// [delta][lse in base 2][bound of |dS|][largest |v|^2], each (heads, tokens_q)
 static size_t packed_stat_bytes(int64_t tokens_q, int64_t heads) {
   return align256((size_t)tokens_q * heads * sizeof(float)) + 256;
 }
-size_t packed_bwd_workspace_size(int64_t tokens_q, int64_t heads) { return 3 * packed_stat_bytes(tokens_q, heads); }
+size_t packed_bwd_workspace_size(int64_t tokens_q, int64_t heads) { return 4 * packed_stat_bytes(tokens_q, heads); }
 
 int packed_forward(const tpo_packed_attention* p, void* o, float* lse, cudaStream_t st) {
   PackedArgs a = args_of(p);
@@ -45,7 +45,10 @@ int packed_backward(const tpo_packed_attention* p, const void* o, const float* l
   a.delta = (float*)ws;
   const bool mma = packed_mma_takes(p->dtype, a, true);
   if (mma) a.lse2 = (float*)((char*)ws + packed_stat_bytes(a.Tq, a.H));
-  if (mma && p->dtype == TPO_F16) a.go_max = (float*)((char*)ws + 2 * packed_stat_bytes(a.Tq, a.H));
+  if (mma && p->dtype == TPO_F16) {
+    a.ds_bound = (float*)((char*)ws + 2 * packed_stat_bytes(a.Tq, a.H));
+    a.v_max = (float*)((char*)ws + 3 * packed_stat_bytes(a.Tq, a.H));
+  }
   int s;
   if (a.Tq > 0 && (s = packed_delta(p->dtype, a, st))) return s;
   return mma ? packed_mma_backward(p->dtype, a, st) : packed_simt_backward(p->dtype, a, st);

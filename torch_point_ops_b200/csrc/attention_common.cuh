@@ -23,7 +23,11 @@ struct PackedArgs {
   const int64_t *off_q, *off_k;
   void *o, *dq, *dk, *dv;
   float *lse, *delta, *lse2;  // lse2: lse in base 2 (backward on the tensor cores), or null
-  float* go_max;  // (H, Tq): largest |go| of each row (fp16 on the tensor cores), or null
+  // fp16 on the tensor cores, else null, each (H, Tq): the length of each row of go, which the dQ
+  // kernel replaces by a bound of the row's |dS|; and, at a cloud's first query and the
+  // first head of a group, the largest |v|^2 of the keys (a cloud without queries has no
+  // dS).
+  float *ds_bound, *v_max;
   int64_t Tq, Tk;
   int B, H, Hk, D, causal;
   float scale;

@@ -423,15 +423,16 @@ __global__ void __launch_bounds__(kThreads) packed_simt_bwd_kernel(const PackedA
   }
 }
 
-// delta = dO . O per (head, token), and where asked for the row's largest |dO| and its
-// log-sum-exp in base 2; lpr lanes per row, vectors of VEC.
+// delta = dO . O per (head, token), and where asked for the row's |dO| (with a zero for the
+// largest |v|^2, which the next kernel raises) and its log-sum-exp in base 2; lpr lanes per
+// row, vectors of VEC.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) packed_delta_kernel(const PackedArgs a, int lpr) {
   const int64_t rows = a.Tq * a.H;
   const int rpb = 256 / lpr, l = threadIdx.x % lpr;
   for (int64_t r0 = (int64_t)blockIdx.x * rpb; r0 < rows; r0 += (int64_t)gridDim.x * rpb) {
     const int64_t r = r0 + threadIdx.x / lpr;
-    float s = 0.f, big = 0.f;
+    float s = 0.f, square = 0.f;
     int64_t tok = 0;
     int head = 0;
     if (r < rows) {
@@ -447,17 +448,20 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const PackedArgs a, i
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           s += x[i] * y[i];
-          big = fmaxf(big, fabsf(y[i]));
+          square += y[i] * y[i];
         }
       }
     }
     for (int x = lpr / 2; x > 0; x >>= 1) {
       s += __shfl_xor_sync(0xffffffffu, s, x);
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
+      square += __shfl_xor_sync(0xffffffffu, square, x);
     }
     if (r < rows && l == 0) {
       a.delta[(int64_t)head * a.Tq + tok] = s;
-      if (a.go_max) a.go_max[(int64_t)head * a.Tq + tok] = big;
+      if (a.ds_bound) {
+        a.ds_bound[(int64_t)head * a.Tq + tok] = sqrtf(square);
+        a.v_max[(int64_t)head * a.Tq + tok] = 0.f;
+      }
       if (a.lse2) a.lse2[(int64_t)head * a.Tq + tok] = a.lse[(int64_t)head * a.Tq + tok] * kLog2e;
     }
   }

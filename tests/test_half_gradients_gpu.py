@@ -72,3 +72,19 @@ def test_one_large_row_among_small_ones():
     some = _gradients(q, k, v, do, [0, 200])
     for name, t in alone.items():
         assert torch.equal(some[name][:200], t), name
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("keys", [300, 50000, 99000])
+def test_gradient_of_values_of_long_clouds(keys, D):
+    # flat rows: every probability is 1 / keys, far below the smallest normal number for many keys
+    rows, each = 2048, 16.0
+    q = torch.zeros(rows, 1, D, device=DEV, dtype=torch.float16)
+    _, k, v, _ = _inputs(keys, 1, 1, D)
+    do = torch.full_like(q, each)
+    dv = _gradients(q, k, v, do, [0, rows], [0, keys])["dv"].double()
+    want = rows * each / keys
+    # one rounding of P, one of the result, each 2^-11 at most; fp32: the log-sum-exp's three roundings
+    # and the sum over the rows (a chain of rows / 8 and a tree)
+    off = 2 * 2.0 ** -11 + (3 * math.log2(keys) + rows / 8 + 64) * R.F
+    assert ((dv - want).abs() <= off * want).all(), float((dv / want - 1).abs().max())

@@ -13,6 +13,7 @@ constexpr unsigned kErrBadOffsets = 4u;
 static __device__ unsigned g_attention_error = 0;  // one per translation unit
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kHalfLift = 12;  // exponent that lifts P of the fp16 backward on the tensor cores
 
 // One packed problem, by value to every kernel.  Strides in elements; the width
 // dimension has stride 1.  o, dq are (Tq, H, D), dk, dv (Tk, Hk, D), lse and
@@ -22,7 +23,7 @@ struct PackedArgs {
   int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, go_st, go_sh;  // token and head strides
   const int64_t *off_q, *off_k;
   void *o, *dq, *dk, *dv;
-  float *lse, *delta, *lse2;  // lse2: lse in base 2 (backward on the tensor cores), or null
+  float *lse, *delta, *lse2;  // lse2: lse in base 2 (backward on the tensor cores; fp16: less kHalfLift), or null
   // fp16 on the tensor cores, else null, each (H, Tq): the length of each row of go, which the dQ
   // kernel replaces by a bound of the row's |dS|; and, at a cloud's first query and the
   // first head of a group, the largest |v|^2 of the keys (a cloud without queries has no

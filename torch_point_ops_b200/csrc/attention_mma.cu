@@ -421,6 +421,13 @@ struct Bwd {
   static constexpr int acc1 = GROUPS * 128, acc2 = acc1 + DP;  // columns; S and dP of group g at 128 g and 128 g + 64
 };
 
+// P of the backward is normalised, about one over the number of keys: fp16 holds it as 2^12 P (the
+// statistics bring the exponent along), or a few 10^4 keys would take it into the subnormal numbers
+// (50000 keys: 1.4e-3 off in dV, against 4.9e-4 that a rounding costs).  2^12 leaves a
+// factor of 16 to the largest fp16.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? (float)(1 << kHalfLift) : 1.f;
+
 // dS of fp16 needs a power of two beside it, or it leaves the type's range at either end.
 // By |dP| <= |dO| |v|, and since P (1 - P) <= 1/4 of the spread of dP is the most that a dS
 // can be, |dS| <= |dO| max |v| / 2 over the cloud's keys.  2^(14 - e) with 2^e the power of
@@ -652,7 +659,7 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
             big = fmaxf(big, a.ds_bound[(int64_t)(head0 + h) * a.Tq + t.b0 + i]);
         big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
       }
-      c = grad_scale(big);
+      c = grad_scale(big) / kLift<T>;
     }
     float row_lse = 0.f, row_delta = 0.f;
     if (!DKV && live) {
@@ -779,7 +786,7 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
     if (!DKV && n > 0) {  // for the kernel of dK and dV, which runs next
       float x, y;
       upk(add2(exact[0], exact[1]), x, y);
-      x += y;
+      x = (x + y) / kLift<T>;
       if (GROUPS == 2) {
         float* other = const_cast<float*>(stats);  // no statistics travel with keys: the space is free
         if (g == 1) other[row] = x;
@@ -803,7 +810,7 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
     for (int which = 0; which < (DKV ? 2 : 1); ++which) {
       if (DKV && GROUPS == 2 && which != g) continue;
       T* op = (T*)(DKV ? (which ? a.dv : a.dk) : a.dq) + at;
-      const float f = which ? 1.f : a.scale / c;
+      const float f = which ? 1.f / kLift<T> : a.scale / (c * kLift<T>);
       const uint32_t acc = (which ? t_2 : t_1) + lane;
 #pragma unroll
       for (int x = 0; x < DP; x += 32) {

@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(256) packed_delta_kernel(const PackedArgs a, i
         a.ds_bound[(int64_t)head * a.Tq + tok] = sqrtf(square);
         a.v_max[(int64_t)head * a.Tq + tok] = 0.f;
       }
-      if (a.lse2) a.lse2[(int64_t)head * a.Tq + tok] = a.lse[(int64_t)head * a.Tq + tok] * kLog2e;
+      if (a.lse2) a.lse2[(int64_t)head * a.Tq + tok] = fmaf(a.lse[(int64_t)head * a.Tq + tok], kLog2e, a.ds_bound ? -(float)kHalfLift : 0.f);
     }
   }
 }

@@ -3,8 +3,8 @@
 //
 // layer_norm and packed_attention are the differentiable entry points: their
 // Autograd kernels run the *_forward op, keep what the *_backward op needs, and
-// raise on a second differentiation.  Only CUDA implementations are registered: a
-// CPU tensor raises.
+// raise on a second differentiation and on a forward-mode derivative.  Only CUDA
+// implementations are registered: a CPU tensor raises.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/all.h>
@@ -37,6 +37,13 @@ int to_dtype(const at::Tensor& t, const char* what) {
 void ok(int status, const char* where) { TORCH_CHECK(status == TPO_OK, where, ": ", tpo_status_string(status)); }
 
 void* stream_of(const at::Tensor& t) { return (void*)at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+// A dual tensor need not require a gradient: without this check its tangent would be dropped below autograd.
+template <typename... Tensors>
+void no_tangents(const char* what, const Tensors&... inputs) {
+  TORCH_CHECK(!(... || (inputs.defined() && inputs._fw_grad(0).defined())), what,
+              ": forward-mode derivatives are not implemented");
+}
 
 // Raises when a gradient that this library computed is differentiated again.
 class FirstOrderOnly : public torch::autograd::Function<FirstOrderOnly> {
@@ -203,6 +210,7 @@ class LayerNormFn : public torch::autograd::Function<LayerNormFn> {
 };
 
 at::Tensor layer_norm_autograd(const at::Tensor& x, const OptTensor& w, const OptTensor& b, double eps) {
+  no_tangents("layer_norm", x, has(w) ? *w : at::Tensor(), has(b) ? *b : at::Tensor());
   const bool grad = at::GradMode::is_enabled() && (x.requires_grad() || (has(w) && w->requires_grad()) ||
                                                    (has(b) && b->requires_grad()));
   if (!grad) {
@@ -363,6 +371,7 @@ class PackedFn : public torch::autograd::Function<PackedFn> {
 
 at::Tensor packed_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& offsets,
                            const OptTensor& offsets_k, bool causal, double scale) {
+  no_tangents("packed_attention", q, k, v);
   if (!(at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))) {
     at::AutoDispatchBelowADInplaceOrView guard;
     static auto op = c10::Dispatcher::singleton()
@@ -407,6 +416,7 @@ at::Tensor cached_cuda(const at::Tensor& q_, const at::Tensor& k_, const at::Ten
 
 at::Tensor cached_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& lengths,
                            double scale) {
+  no_tangents("cached_attention", q, k, v);
   TORCH_CHECK(!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad()),
               "cached_attention has no backward pass: call it under torch.no_grad(), or train with packed_attention");
   at::AutoDispatchBelowADInplaceOrView guard;

@@ -8,8 +8,10 @@
 // A few operations per element: HBM traffic is the bound (forward 2 passes over
 // (R, C), backward 3).  So a row is read once and stays in registers for both
 // moments and the result; the variance is the centred second pass over those
-// registers, which loses nothing when |mean| >> std.  All sums are fp32 (fp64 for
-// fp64 rows); outputs are rounded once.
+// registers.  That pass also sums the centred values: what the mean's rounding left
+// (up to some 2^-20 |mean|, which 1 / std magnifies) is taken out of y, the
+// variance and the mean that the backward reads.  All sums are fp32 (fp64 for fp64
+// rows); outputs are rounded once.
 //
 // Measured (B200, GB/s of the passes above; a plain copy moves 6555): forward 65536 x 512 fp32
 // 42.6 us (6300), 32768 x 1024 bf16 25.8 us (5210: issue slots, conversions), 10007 x 771
@@ -43,12 +45,36 @@ __device__ __forceinline__ A row_sum(A v, A* red, int bar) {
   return v;
 }
 
+// Two such sums with one barrier.
+template <int TPR, typename A>
+__device__ __forceinline__ void row_sums(A& v, A& w, A* red_v, A* red_w, int bar) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    v += __shfl_xor_sync(0xffffffffu, v, o);
+    w += __shfl_xor_sync(0xffffffffu, w, o);
+  }
+  if (TPR > 32) {
+    const int wid = (threadIdx.x % TPR) / 32;
+    if (threadIdx.x % 32 == 0) red_v[wid] = v, red_w[wid] = w;
+    asm volatile("bar.sync %0, %1;" ::"r"(bar), "n"(TPR) : "memory");
+    v = red_v[0], w = red_w[0];
+#pragma unroll
+    for (int i = 1; i < TPR / 32; ++i) v += red_v[i], w += red_w[i];
+  }
+}
+
 template <typename A>
 __device__ __forceinline__ A inv_std(A var, A eps);
 template <>
 __device__ __forceinline__ float inv_std<float>(float var, float eps) { return rsqrtf(var + eps); }  // within 2 ulp
 template <>
 __device__ __forceinline__ double inv_std<double>(double var, double eps) { return rsqrt(var + eps); }
+
+// var - part where that is positive, else 0; a variance beyond the type's range stays infinite.
+template <typename A>
+__device__ __forceinline__ A without(A var, A part) {
+  return part < var ? var - part : var < (A)INFINITY ? (A)0 : var;
+}
 
 // A thread's vectors of a row (vector i: columns (i * TPR + t) * VEC on) as accumulators.
 // Vectors beyond column C are zeros: they are cleared once and never loaded, so no
@@ -103,7 +129,7 @@ __global__ void __launch_bounds__(TPR* RPB)
   // 16 bits: conversions keep the issue slots busy, and the registers of a second
   // row cost more warps than it brings (measured, 32768 x 1024: 26.6 against 25.8 us).
   constexpr bool AHEAD = sizeof(T) != 2;
-  __shared__ A red[RPB][4][TPR / 32];
+  __shared__ A red[RPB][6][TPR / 32];
   const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
   const A eps = (A)eps_, inv_c = (A)1 / (A)C;
   const int64_t step = (int64_t)gridDim.x * RPB;
@@ -140,6 +166,7 @@ __global__ void __launch_bounds__(TPR* RPB)
 #pragma unroll
     for (int e = 0; e < EPT; ++e) s += v[e];
     const A mean = row_sum<TPR>(s, red[g][phase], g + 1) * inv_c;
+    A rest = 0;
     s = 0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -147,13 +174,16 @@ __global__ void __launch_bounds__(TPR* RPB)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         v[i * VEC + j] -= m;
+        rest += v[i * VEC + j];
         s += v[i * VEC + j] * v[i * VEC + j];
       }
     }
-    const A rstd = inv_std<A>(row_sum<TPR>(s, red[g][phase + 1], g + 1) * inv_c, eps);
-    phase ^= 2;
+    row_sums<TPR>(rest, s, red[g][phase + 1], red[g][phase + 2], g + 1);
+    rest *= inv_c;  // what the mean's rounding left
+    const A rstd = inv_std<A>(without(s * inv_c, rest * rest), eps), shift = -rest * rstd;
+    phase ^= 3;
     if (t == 0 && mean_out) {
-      mean_out[row] = mean;
+      mean_out[row] = mean + rest;
       rstd_out[row] = rstd;
     }
 #pragma unroll
@@ -163,7 +193,7 @@ __global__ void __launch_bounds__(TPR* RPB)
       unpack<VEC, 1>(wk, reinterpret_cast<const Pack<W, VEC>(&)[1]>(SHARED ? ws[i * TPR + t] : wv[i]));
       unpack<VEC, 1>(bk, reinterpret_cast<const Pack<W, VEC>(&)[1]>(SHARED ? bs[i * TPR + t] : bv[i]));
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) o[j] = v[i * VEC + j] * rstd * wk[j] + bk[j];
+      for (int j = 0; j < VEC; ++j) o[j] = (v[i * VEC + j] * rstd + shift) * wk[j] + bk[j];
       if (c < C) store_vec<VEC>(y + row * C + c, o);
     }
     if (AHEAD) {
@@ -318,7 +348,7 @@ __global__ void __launch_bounds__(512)
                        T* __restrict__ y, Acc<T>* __restrict__ mean_out,
                        Acc<T>* __restrict__ rstd_out) {
   using A = Acc<T>;
-  __shared__ A red[4][16];
+  __shared__ A red[6][16];
   const A inv_c = (A)1 / (A)C;
   int phase = 0;
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
@@ -326,20 +356,24 @@ __global__ void __launch_bounds__(512)
     A s = 0;
     for (int64_t c = threadIdx.x; c < C; c += 512) s += to_acc(xr[c]);
     const A mean = row_sum<512>(s, red[phase], 1) * inv_c;
+    A rest = 0;
     s = 0;
     for (int64_t c = threadIdx.x; c < C; c += 512) {
       const A d = to_acc(xr[c]) - mean;
+      rest += d;
       s += d * d;
     }
-    const A rstd = inv_std<A>(row_sum<512>(s, red[phase + 1], 1) * inv_c, (A)eps_);
-    phase ^= 2;
+    row_sums<512>(rest, s, red[phase + 1], red[phase + 2], 1);
+    rest *= inv_c;
+    const A rstd = inv_std<A>(without(s * inv_c, rest * rest), (A)eps_), shift = -rest * rstd;
+    phase ^= 3;
     if (threadIdx.x == 0 && mean_out) {
-      mean_out[row] = mean;
+      mean_out[row] = mean + rest;
       rstd_out[row] = rstd;
     }
     for (int64_t c = threadIdx.x; c < C; c += 512) {
       const A wv = w ? to_acc(w[c]) : (A)1, bv = b ? to_acc(b[c]) : (A)0;
-      y[row * C + c] = from_acc<T>((to_acc(xr[c]) - mean) * rstd * wv + bv);
+      y[row * C + c] = from_acc<T>(((to_acc(xr[c]) - mean) * rstd + shift) * wv + bv);
     }
   }
 }

@@ -280,7 +280,9 @@ TPO_API int tpo_layer_norm_bwd(int dtype, int wdtype, const void* x, int64_t x_s
  * zeros and lse -inf; its gradients are zeros.  A cloud's result depends on
  * that cloud's tokens alone, whatever its neighbours hold.
  * dtype: TPO_F32, TPO_F16, TPO_BF16; width 1 to 256.  Strides are in elements, the
- * width dimension has stride 1.  Sums are fp32; for 16-bit types the probabilities
+ * width dimension has stride 1.  Inputs and outputs may lie at any address of their
+ * type; 16-bit problems with a width of whole 16 bytes up to 128 and all of them on 16 bytes
+ * run on the tensor cores, others on the FP32 pipe.  Sums are fp32; for 16-bit types the probabilities
  * are rounded to that type before they multiply v (and grad_o), as is dS before it
  * multiplies q; dS multiplies k as the sum of two values of that type. */
 typedef struct tpo_packed_attention {

@@ -891,8 +891,10 @@ bool rows16(const void* p, int64_t s1, int64_t s2) {
 }  // namespace
 
 bool packed_mma_takes(int dtype, const PackedArgs& a, bool backward) {
+  // every row of inputs and outputs starts on 16 bytes (outputs are contiguous; null ones are not written)
+  const bool out = backward ? rows16(a.dq, 0, 0) && rows16(a.dk, 0, 0) && rows16(a.dv, 0, 0) : rows16(a.o, 0, 0);
   return (dtype == TPO_F16 || dtype == TPO_BF16) && a.D % 8 == 0 && a.D <= 128 && rows16(a.q, a.q_st, a.q_sh) &&
-         rows16(a.k, a.k_st, a.k_sh) && rows16(a.v, a.v_st, a.v_sh) && (!backward || rows16(a.go, a.go_st, a.go_sh));
+         rows16(a.k, a.k_st, a.k_sh) && rows16(a.v, a.v_st, a.v_sh) && out && (!backward || rows16(a.go, a.go_st, a.go_sh));
 }
 
 int packed_mma_forward(int dtype, const PackedArgs& a, cudaStream_t st) {

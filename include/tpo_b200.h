@@ -72,6 +72,10 @@ enum tpo_device_errors {
   TPO_DEVERR_MMA_TIMEOUT = 8   /* packed attention: a wait inside a block gave up */
 };
 TPO_API int tpo_device_error_flags(unsigned* flags, int clear);
+/* Sets `flags` in the word of one of the library's kernel files (unit 0, 1, ... until
+ * TPO_ERR_INVALID_ARGUMENT), as its kernels do when they give up (synchronous): what a
+ * caller does on an error can be tested without one. */
+TPO_API int tpo_device_error_raise(int unit, unsigned flags);
 
 /* ------------------------------------------------------------------------- */
 /* Chamfer distance forward.  Replaces chamfer_cuda_forward

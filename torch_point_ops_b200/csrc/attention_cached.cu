@@ -741,4 +741,6 @@ int cached_attention(int dtype, const void* q, const int64_t* q_stride, const vo
   }
 }
 
+int attention_cached_error_word(unsigned** word) { return attention_error_word(word); }
+
 }  // namespace tpo

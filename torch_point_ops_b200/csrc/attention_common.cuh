@@ -10,7 +10,7 @@ namespace tpo {
 // Set by a kernel that met offsets that decrease or leave [0, tokens]
 // (TPO_DEVERR_BAD_OFFSETS); what it reads and writes stays clamped.
 constexpr unsigned kErrBadOffsets = 4u;
-static __device__ unsigned g_attention_error = 0;  // one per translation unit
+static __device__ unsigned g_attention_error = 0;  // one per translation unit: each is in capi.cu's table
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kHalfLift = 12;  // exponent that lifts P of the fp16 backward on the tensor cores
@@ -134,11 +134,8 @@ __device__ __forceinline__ Tile find_tile(const int64_t* off, int64_t T, const i
   return t;
 }
 
-inline int read_attention_error(unsigned* out, bool clear) {
-  int s = cuda_status(cudaMemcpyFromSymbol(out, g_attention_error, sizeof(unsigned)));
-  if (s || !clear) return s;
-  const unsigned zero = 0;
-  return cuda_status(cudaMemcpyToSymbol(g_attention_error, &zero, sizeof(unsigned)));
+static inline int attention_error_word(unsigned** word) {  // of this translation unit
+  return cuda_status(cudaGetSymbolAddress((void**)word, g_attention_error));
 }
 
 int packed_simt_forward(int dtype, const PackedArgs& a, cudaStream_t st);

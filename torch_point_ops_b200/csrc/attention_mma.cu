@@ -907,6 +907,6 @@ int packed_mma_backward(int dtype, const PackedArgs& a, cudaStream_t st) {
   return a.D <= 64 ? bwd<__nv_bfloat16, 64>(a, st) : bwd<__nv_bfloat16, 128>(a, st);
 }
 
-int attention_mma_error_flags(unsigned* out, bool clear) { return read_attention_error(out, clear); }
+int attention_mma_error_word(unsigned** word) { return attention_error_word(word); }
 
 }  // namespace tpo

@@ -572,6 +572,6 @@ int packed_simt_forward(int dtype, const PackedArgs& a, cudaStream_t st) { TPO_D
 int packed_simt_backward(int dtype, const PackedArgs& a, cudaStream_t st) { TPO_DISPATCH(bwd_typed) }
 int packed_delta(int dtype, const PackedArgs& a, cudaStream_t st) { TPO_DISPATCH(delta_typed) }
 
-int attention_simt_error_flags(unsigned* out, bool clear) { return read_attention_error(out, clear); }
+int attention_simt_error_word(unsigned** word) { return attention_error_word(word); }
 
 }  // namespace tpo

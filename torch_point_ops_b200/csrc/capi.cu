@@ -47,16 +47,33 @@ const char* tpo_status_string(int status) {
   return "unknown status";
 }
 
+// Every file whose kernels set error flags.
+static int (*const kErrorWords[])(unsigned**) = {chamfer_error_word,        fps_error_word,           knn_error_word,
+                                                 attention_simt_error_word, attention_mma_error_word, attention_cached_error_word};
+
 int tpo_device_error_flags(unsigned* flags, int clear) {
   if (!flags) return fail(TPO_ERR_INVALID_ARGUMENT, "device_error_flags: null output");
-  unsigned a = 0, b = 0, c = 0, d = 0, e = 0;
-  int s = device_error_flags(&a, clear != 0);
-  if (!s) s = fps_device_error_flags(&b, clear != 0);
-  if (!s) s = knn_device_error_flags(&c, clear != 0);
-  if (!s) s = attention_simt_error_flags(&d, clear != 0);
-  if (!s) s = attention_mma_error_flags(&e, clear != 0);
-  *flags = a | b | c | d | e;
-  return s;
+  *flags = 0;
+  for (auto word_of : kErrorWords) {
+    unsigned *word = nullptr, value = 0;
+    const unsigned zero = 0;
+    int s = word_of(&word);
+    if (!s) s = cuda_status(cudaMemcpy(&value, word, sizeof value, cudaMemcpyDeviceToHost));
+    if (!s && clear) s = cuda_status(cudaMemcpy(word, &zero, sizeof zero, cudaMemcpyHostToDevice));
+    if (s) return s;
+    *flags |= value;
+  }
+  return TPO_OK;
+}
+
+int tpo_device_error_raise(int unit, unsigned flags) {
+  if (unit < 0 || unit >= (int)(sizeof kErrorWords / sizeof *kErrorWords))
+    return fail(TPO_ERR_INVALID_ARGUMENT, "device_error_raise: no such unit");
+  unsigned *word = nullptr, value = 0;
+  int s = kErrorWords[unit](&word);
+  if (!s) s = cuda_status(cudaMemcpy(&value, word, sizeof value, cudaMemcpyDeviceToHost));
+  value |= flags;
+  return s ? s : cuda_status(cudaMemcpy(word, &value, sizeof value, cudaMemcpyHostToDevice));
 }
 
 int tpo_chamfer_key_bytes(int dtype) {

@@ -1245,11 +1245,6 @@ int chamfer_bwd_from_keys(int dtype, int flags, const void* x1, const void* x2, 
                     reduction, (float*)gx1, (float*)gx2);
 }
 
-int device_error_flags(unsigned* out, bool clear) {
-  int s = cuda_status(cudaMemcpyFromSymbol(out, g_fwd_device_error, sizeof(unsigned)));
-  if (s || !clear) return s;
-  const unsigned zero = 0;
-  return cuda_status(cudaMemcpyToSymbol(g_fwd_device_error, &zero, sizeof(unsigned)));
-}
+int chamfer_error_word(unsigned** word) { return cuda_status(cudaGetSymbolAddress((void**)word, g_fwd_device_error)); }
 
 }  // namespace tpo

@@ -741,11 +741,6 @@ int fps_forward(int dtype, const void* pts, int64_t B, int64_t P, int64_t S, int
   return TPO_ERR_INVALID_ARGUMENT;
 }
 
-int fps_device_error_flags(unsigned* out, bool clear) {
-  int s = cuda_status(cudaMemcpyFromSymbol(out, g_fps_device_error, sizeof(unsigned)));
-  if (s || !clear) return s;
-  const unsigned zero = 0;
-  return cuda_status(cudaMemcpyToSymbol(g_fps_device_error, &zero, sizeof(unsigned)));
-}
+int fps_error_word(unsigned** word) { return cuda_status(cudaGetSymbolAddress((void**)word, g_fps_device_error)); }
 
 }  // namespace tpo

@@ -1297,11 +1297,6 @@ int knn_gather_backward(int dtype, const void* gout, const int64_t* idx, const i
   return gather_dispatch(true, dtype, gout, idx, lengths, N, M, U, L, K, gx, st);
 }
 
-int knn_device_error_flags(unsigned* out, bool clear) {
-  int s = cuda_status(cudaMemcpyFromSymbol(out, g_knn_device_error, sizeof(unsigned)));
-  if (s || !clear) return s;
-  const unsigned zero = 0;
-  return cuda_status(cudaMemcpyToSymbol(g_knn_device_error, &zero, sizeof(unsigned)));
-}
+int knn_error_word(unsigned** word) { return cuda_status(cudaGetSymbolAddress((void**)word, g_knn_device_error)); }
 
 }  // namespace tpo

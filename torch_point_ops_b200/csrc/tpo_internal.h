@@ -67,14 +67,18 @@ int chamfer_bwd_from_keys(int dtype, int flags, const void* x1, const void* x2, 
 int fill_prefetch(void* d0, size_t n0, void* d1, size_t n1, unsigned char value, const void* p0,
                   size_t m0, const void* p1, size_t m1, cudaStream_t st, int value1 = -1);
 
-// Reads (and optionally clears) the device-side error flags of this device.
-int device_error_flags(unsigned* out, bool clear);
+// The current device's address of the word in which a file's kernels set error flags; capi.cu has them all
+// in one table.
+int chamfer_error_word(unsigned** word);
+int fps_error_word(unsigned** word);
+int knn_error_word(unsigned** word);
+int attention_simt_error_word(unsigned** word);
+int attention_mma_error_word(unsigned** word);
+int attention_cached_error_word(unsigned** word);
 
 size_t fps_workspace_size(int dtype, int64_t B, int64_t P);
 int fps_forward(int dtype, const void* pts, int64_t B, int64_t P, int64_t S, int64_t* idx,
                 void* ws, size_t ws_bytes, cudaStream_t st);
-int fps_device_error_flags(unsigned* out, bool clear);
-int knn_device_error_flags(unsigned* out, bool clear);
 int gather_points_forward(int dtype, const void* pts, const int64_t* idx, int64_t N, int64_t C,
                           int64_t P, int64_t M, void* out, cudaStream_t st);
 int gather_points_backward(int dtype, const void* gout, const int64_t* idx, int64_t N, int64_t C,
@@ -99,8 +103,6 @@ int cached_attention(int dtype, const void* q, const int64_t* q_stride, const vo
                      const int64_t* k_stride, const void* v, const int64_t* v_stride,
                      const int64_t* lengths, int64_t N, int64_t P, int64_t H, int64_t Hk, int64_t D,
                      float scale, void* o, void* ws, cudaStream_t st);
-int attention_simt_error_flags(unsigned* out, bool clear);
-int attention_mma_error_flags(unsigned* out, bool clear);
 
 // Launches `kern` with programmatic stream serialisation allowed (see pdl_wait).
 template <typename... KArgs, typename... Args>

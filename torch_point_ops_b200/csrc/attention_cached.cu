@@ -3,8 +3,9 @@
 //
 //   s_j = scale * q . k_j (j < length),  o = sum_j exp(s_j - max) v_j / sum_j exp(s_j - max)
 //
-// Two to four operations per byte of cache: HBM is the bound, so every cached
-// token is read once for all query heads of its group.  The key axis is cut into chunks
+// Two to four operations per byte of cache: HBM is the bound, so a cached token is read
+// once for all query heads of its group, up to 16 of them in the matrix kernel and 4 in the
+// other; larger groups read it ceil(group / 16) or ceil(group / 4) times.  The key axis is cut into chunks
 // of a fixed number of tokens (chosen by the host from N, Hk and P, so no length is copied
 // to the host); a block takes one chunk of one (cloud, kv head).  Up to 8 short chunks are a
 // thread-block cluster, which joins them through its shared memory in chunk order.  More
@@ -699,9 +700,13 @@ int cached_typed(CachedArgs a, cudaStream_t st) {
     }
   }
   if (aligned16<T>(a)) {
-    if (a.D <= 16 * V) s = simt_group<T, V, 16, 1>(a, st);
-    else if (a.D <= 32 * V) s = simt_group<T, V, 32, 1>(a, st);
-    else s = simt_group<T, V, 32, 256 / (32 * V)>(a, st);
+    if constexpr (sizeof(T) == 2) {  // wider than 128, or the matrix kernel had it
+      s = simt_group<T, V, 32, 1>(a, st);
+    } else {
+      if (a.D <= 16 * V) s = simt_group<T, V, 16, 1>(a, st);
+      else if (a.D <= 32 * V) s = simt_group<T, V, 32, 1>(a, st);
+      else s = simt_group<T, V, 32, 2>(a, st);
+    }
   } else {
     if (a.D <= 64) s = simt_group<T, 1, 32, 2>(a, st);
     else if (a.D <= 128) s = simt_group<T, 1, 32, 4>(a, st);

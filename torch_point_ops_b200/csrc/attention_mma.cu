@@ -2,8 +2,9 @@
 // multiple of 8 up to 128, rows on 16-byte boundaries.
 //
 // All products are tcgen05 with fp32 accumulators in tensor memory (TMEM).  A block has
-// row warps (a thread owns a row of the score tile), two copy warps and one thread that
-// issues products; tiles travel through a ring in shared memory.
+// row warps (a thread owns a row of the score tile), two copy warps and a warp that issues
+// products (two warps in the backward), one elected lane of it; tiles travel through a ring in
+// shared memory.
 //
 // The tensor cores take no wider operand beside 16-bit ones.  P is rounded to 16 bits
 // before it multiplies V (and dO): that adds about as much error as the rounding of the
@@ -141,7 +142,7 @@ struct Fwd {
   static constexpr int launch_regs = TILES == 2 ? 168 : 128;
   static_assert(TILES * 128 * row_regs + 128 * other_regs <= threads * launch_regs, "register split");
   static constexpr int tile = kTile * DP * 2;
-  static constexpr int stages = DP == 128 ? 5 : 5;
+  static constexpr int stages = 5;
   static constexpr int bars = (TILES + stages) * tile;
   static constexpr int smem = bars + 256 + 1024;  // + alignment of the base
   static constexpr int tmem = TILES * 256;

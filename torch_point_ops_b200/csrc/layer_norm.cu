@@ -76,6 +76,27 @@ __device__ __forceinline__ A without(A var, A part) {
   return part < var ? var - part : var < (A)INFINITY ? (A)0 : var;
 }
 
+// Two values at a time: fp32 has packed instructions, which take half of the issue slots.
+struct Doubles { double x, y; };
+using tpo::add2;
+using tpo::fma2;
+using tpo::sub2;
+template <typename A>
+using Two = std::conditional_t<std::is_same<A, float>::value, u64, Doubles>;
+__device__ __forceinline__ u64 two(float x, float y) { return pk(x, y); }
+__device__ __forceinline__ Doubles two(double x, double y) { return {x, y}; }
+__device__ __forceinline__ void apart(u64 v, float& x, float& y) { upk(v, x, y); }
+__device__ __forceinline__ void apart(Doubles v, double& x, double& y) { x = v.x, y = v.y; }
+__device__ __forceinline__ Doubles add2(Doubles a, Doubles b) { return {a.x + b.x, a.y + b.y}; }
+__device__ __forceinline__ Doubles sub2(Doubles a, Doubles b) { return {a.x - b.x, a.y - b.y}; }
+__device__ __forceinline__ Doubles fma2(Doubles a, Doubles b, Doubles c) { return {fma(a.x, b.x, c.x), fma(a.y, b.y, c.y)}; }
+template <typename A>
+__device__ __forceinline__ A both(Two<A> v) {
+  A x, y;
+  apart(v, x, y);
+  return x + y;
+}
+
 // A thread's vectors of a row (vector i: columns (i * TPR + t) * VEC on) as accumulators.
 // Vectors beyond column C are zeros: they are cleared once and never loaded, so no
 // element needs a test of its own.
@@ -161,41 +182,46 @@ __global__ void __launch_bounds__(TPR* RPB)
   while (row < rows) {
     const int64_t next = row + step;
     if (AHEAD && next < rows) load_row<VEC, TPR, EPT>(nxt, x + next * xs, t, C);
-    A v[EPT], s = 0;
-    unpack(v, cur);
+    Two<A> v[EPT / 2], sum, squares;
+    {
+      A one[EPT];
+      unpack(one, cur);
 #pragma unroll
-    for (int e = 0; e < EPT; ++e) s += v[e];
-    const A mean = row_sum<TPR>(s, red[g][phase], g + 1) * inv_c;
-    A rest = 0;
-    s = 0;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const A m = (i * TPR + t) * VEC < C ? mean : (A)0;  // vectors beyond C are no part of the variance
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        v[i * VEC + j] -= m;
-        rest += v[i * VEC + j];
-        s += v[i * VEC + j] * v[i * VEC + j];
-      }
+      for (int e = 0; e < EPT / 2; ++e) v[e] = two(one[2 * e], one[2 * e + 1]);
     }
-    row_sums<TPR>(rest, s, red[g][phase + 1], red[g][phase + 2], g + 1);
+    sum = v[0];
+#pragma unroll
+    for (int e = 1; e < EPT / 2; ++e) sum = add2(sum, v[e]);
+    const A mean = row_sum<TPR>(both<A>(sum), red[g][phase], g + 1) * inv_c;
+    sum = squares = two((A)0, (A)0);
+#pragma unroll
+    for (int e = 0; e < EPT / 2; ++e) {
+      // vectors beyond C are no part of the variance
+      const bool in0 = (2 * e / VEC * TPR + t) * VEC < C, in1 = ((2 * e + 1) / VEC * TPR + t) * VEC < C;
+      v[e] = sub2(v[e], two(in0 ? mean : (A)0, in1 ? mean : (A)0));
+      sum = add2(sum, v[e]);
+      squares = fma2(v[e], v[e], squares);
+    }
+    A rest = both<A>(sum), var = both<A>(squares);
+    row_sums<TPR>(rest, var, red[g][phase + 1], red[g][phase + 2], g + 1);
     rest *= inv_c;  // what the mean's rounding left
-    const A rstd = inv_std<A>(without(s * inv_c, rest * rest), eps), shift = -rest * rstd;
+    const A rstd = inv_std<A>(without(var * inv_c, rest * rest), eps), shift = -rest * rstd;
     phase ^= 3;
     if (t == 0 && mean_out) {
       mean_out[row] = mean + rest;
       rstd_out[row] = rstd;
     }
+    A o[EPT], wk[EPT], bk[EPT];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int c = (i * TPR + t) * VEC;
-      A o[VEC], wk[VEC], bk[VEC];
-      unpack<VEC, 1>(wk, reinterpret_cast<const Pack<W, VEC>(&)[1]>(SHARED ? ws[i * TPR + t] : wv[i]));
-      unpack<VEC, 1>(bk, reinterpret_cast<const Pack<W, VEC>(&)[1]>(SHARED ? bs[i * TPR + t] : bv[i]));
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) o[j] = (v[i * VEC + j] * rstd + shift) * wk[j] + bk[j];
-      if (c < C) store_vec<VEC>(y + row * C + c, o);
+      unpack<VEC, 1>(reinterpret_cast<A(&)[VEC]>(wk[i * VEC]), reinterpret_cast<const Pack<W, VEC>(&)[1]>(SHARED ? ws[i * TPR + t] : wv[i]));
+      unpack<VEC, 1>(reinterpret_cast<A(&)[VEC]>(bk[i * VEC]), reinterpret_cast<const Pack<W, VEC>(&)[1]>(SHARED ? bs[i * TPR + t] : bv[i]));
     }
+#pragma unroll
+    for (int e = 0; e < EPT / 2; ++e)
+      apart(fma2(fma2(v[e], two(rstd, rstd), two(shift, shift)), two(wk[2 * e], wk[2 * e + 1]), two(bk[2 * e], bk[2 * e + 1])),
+            o[2 * e], o[2 * e + 1]);
+    store_row<VEC, TPR, EPT>(y + row * C, o, t, C);
     if (AHEAD) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) cur[i] = nxt[i];

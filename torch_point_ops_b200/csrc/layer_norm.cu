@@ -13,10 +13,13 @@
 // variance and the mean that the backward reads.  All sums are fp32 (fp64 for fp64
 // rows); outputs are rounded once.
 //
-// Measured (B200, GB/s of the passes above; a plain copy moves 6555): forward 65536 x 512 fp32
-// 42.6 us (6300), 32768 x 1024 bf16 25.8 us (5210: issue slots, conversions), 10007 x 771
-// fp16 11.3 us (2720: one element per load); backward 67.7 us (5950), 39.3 us (5120),
-// 16.3 us (2840).
+// Measured (B200, GB/s of the passes above; a plain copy moves 6555), inputs where the last
+// call left them: forward 65536 x 512 fp32 42.9 us (6260), 32768 x 1024 bf16 24.3 us (5520: issue
+// slots, conversions), 10007 x 771 fp16 12.0 us (2580: one element per load); backward 65.0 us
+// (6200), 38.7 us (5200), 16.2 us (2860).  With L2 flushed before each call: fp64 8192 x 1024
+// forward 34.8 us (3860), backward 103 us (1950: registers, spills); rows wider than 8192
+// loop over single elements: 4096 x 16384 bf16 forward 119 us (2260), backward 251 us
+// (1600), 4096 x 9000 fp32 100 us (2930) and 174 us (2540).
 #include "tpo_internal.h"
 #include "tpo_types.cuh"
 
@@ -148,16 +151,17 @@ __global__ void __launch_bounds__(TPR* RPB)
   constexpr int NV = EPT / VEC;
   // 32 and 64 bits: the next row is on its way while this one is reduced and written.
   // 16 bits: conversions keep the issue slots busy, and the registers of a second
-  // row cost more warps than it brings (measured, 32768 x 1024: 26.6 against 25.8 us).
+  // row cost more warps than it brings (measured, bf16, 32768 x 1024: 25.3 against 24.3 us).
   constexpr bool AHEAD = sizeof(T) != 2;
   __shared__ A red[RPB][6][TPR / 32];
   const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
   const A eps = (A)eps_, inv_c = (A)1 / (A)C;
   const int64_t step = (int64_t)gridDim.x * RPB;
   int64_t row = (int64_t)blockIdx.x * RPB + g;
-  // Whole vectors of 16-bit rows: the parameters wait in shared memory, their registers
-  // would cost a third of the warps (measured, 32768 x 1024: 30.1 against 25.8 us).
-  constexpr bool SHARED = sizeof(T) == 2 && VEC == 8 && EPT > 8 && 2 * NV * TPR * sizeof(Pack<W, VEC>) <= 40960;
+  // Whole vectors of 16-bit rows wider than 512: the parameters wait in shared memory, their registers
+  // would cost a third of the warps (measured, bf16: 32768 x 1024 29.7 against 24.3 us, 32768 x
+  // 2048 57.7 against 50.4; narrower rows have few: 32768 x 512 10.0 against 12.0 with shared memory).
+  constexpr bool SHARED = sizeof(T) == 2 && VEC == 8 && TPR * EPT > 512 && 2 * NV * TPR * sizeof(Pack<W, VEC>) <= 40960;
   __shared__ Pack<W, VEC> ws[SHARED ? NV * TPR : 1], bs[SHARED ? NV * TPR : 1];
   Pack<T, VEC> cur[NV], nxt[NV];
   Pack<W, VEC> wv[NV], bv[NV];

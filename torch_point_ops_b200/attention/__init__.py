@@ -68,7 +68,7 @@ def packed_attention(
     Returns:
         (T, H, D).  A query that sees no key, and a token outside of every
         cloud, gives zeros and has zero gradients.  Differentiable once in q, k,
-        v, with the same bits in every run.  Nothing from another cloud enters a
+        v (reverse mode), with the same bits in every run.  Nothing from another cloud enters a
         result; within a causal cloud a value that is not finite may
         reach earlier queries of its own tile of 128 keys.
     """

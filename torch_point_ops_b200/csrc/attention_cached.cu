@@ -16,8 +16,9 @@
 //
 // Measured (B200, bf16, width 128): 64 clouds of 4096 tokens, 32 heads over 8: 180 us, 5.97
 // TB/s of cache; one cloud of 131072 tokens, 16 heads over 4: 50 us, 5.4 TB/s (a plain copy
-// moves 6.56); fp32, 8 ragged clouds of up to 16384 tokens: 60 us, 4.2 TB/s.  What is left is
-// the start of the blocks, the join (4 us) and, in fp32, load latency.  One cloud of 256 tokens,
+// moves 6.56); fp32, 32 clouds of 4096 tokens: 32 heads over 8 256 us, 4.2 TB/s, 32 over 32
+// 644 us, 6.7 TB/s (grouped heads: scores and sums per loaded byte); bf16 width 256 (the FP32
+// pipe): 496 us, 2.2 TB/s.  What is left is the start of the blocks and the join (4 us).  One cloud of 256 tokens,
 // 8 heads of width 64: 4.8 us, a chain of latencies.
 #include "attention_common.cuh"
 #include "tcgen05.cuh"  // asynchronous copies

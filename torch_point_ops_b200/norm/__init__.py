@@ -44,8 +44,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor = None, bias: torch.Tensor 
         eps: added to the (biased) variance
     Returns:
         (..., C), x's dtype.  Moments and sums are held in float32 (float64 for
-        float64); differentiable once in x, weight and bias, with the same bits
-        in every run.
+        float64); differentiable once in x, weight and bias (reverse mode), with
+        the same bits in every run.
     """
     return _ops.layer_norm(x, weight, bias, eps)
 

@@ -88,3 +88,36 @@ def test_gradient_of_values_of_long_clouds(keys, D):
     # and the sum over the rows (a chain of rows / 8 and a tree)
     off = 2 * 2.0 ** -11 + (3 * math.log2(keys) + rows / 8 + 64) * R.F
     assert ((dv - want).abs() <= off * want).all(), float((dv / want - 1).abs().max())
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("before", [0, 300])
+def test_keys_that_are_not_seen_leave_the_scale_alone(before, D):
+    # later keys of a causal cloud hold values 2^12 times as large: tiles of queries that see none of them
+    q, k, v, do = _inputs(700, 2, 1, D)
+    rows = 700 - before  # so many queries, the last ones
+    off, off_k = [0, rows], [0, 700]
+    args = lambda v: (q[:rows], k, v, do[:rows], off, off_k, True)
+    base = _gradients(*args(v))["dq"]
+    last = 512 - before  # queries below see keys below 512 only, and start tiles of their own
+    v = v.clone()
+    v[512:] *= 2.0 ** 12
+    seen = last // 128 * 128
+    got = _gradients(*args(v))["dq"]
+    assert seen > 0 and torch.equal(got[:seen], base[:seen])
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows,keys", [(1, 3000), (3, 1000), (5, 130), (200, 5000)])
+def test_few_rows_over_many_tiles_of_large_values(rows, keys, D):
+    # the largest value of the last tile counts, however few queries there are
+    q, k, v, do = _inputs(keys, 2, 1, D)
+    v[-1] = 4000.0
+    v[-2] = -4000.0
+    k[-2:] = 3 * q[0, 0]  # and it is attended to
+    do = torch.full_like(do, 2.0 ** -9)
+    ref = R.packed(q[:rows], k, v, [0, rows], [0, keys], True, 1 / math.sqrt(D), do[:rows])
+    for name, t in _gradients(q[:rows], k, v, do[:rows], [0, rows], [0, keys], True).items():
+        assert torch.isfinite(t).all(), name
+        R.check(t, ref[name], name)

@@ -25,9 +25,9 @@ struct PackedArgs {
   void *o, *dq, *dk, *dv;
   float *lse, *delta, *lse2;  // lse2: lse in base 2 (backward on the tensor cores; fp16: less kHalfLift), or null
   // fp16 on the tensor cores, else null, each (H, Tq): the length of each row of go, which the dQ
-  // kernel replaces by a bound of the row's |dS|; and, at a cloud's first query and the
-  // first head of a group, the largest |v|^2 of the keys (a cloud without queries has no
-  // dS).
+  // kernel replaces by a bound of the row's |dS|; and the largest |v|^2 of each tile of keys, in
+  // the row of a group's first head: tile i of a cloud at its query i, those beyond the last query
+  // there too (a cloud without queries has no dS).
   float *ds_bound, *v_max;
   int64_t Tq, Tk;
   int B, H, Hk, D, causal;

@@ -431,16 +431,17 @@ constexpr float kLift = std::is_same<T, __half>::value ? (float)(1 << kHalfLift)
 
 // dS of fp16 needs a power of two beside it, or it leaves the type's range at either end.
 // By |dP| <= |dO| |v|, and since P (1 - P) <= 1/4 of the spread of dP is the most that a dS
-// can be, |dS| <= |dO| max |v| / 2 over the cloud's keys.  2^(14 - e) with 2^e the power of
-// two at or below that product (without the half) brings |dS| below 2^14: a factor of
-// four from the largest fp16 for what P and delta are off, and all of the range below for small P
-// (undone when acc1 leaves).
+// can be, |dS| <= |dO| max |v| / 2 over the keys that the row's tile meets.  2^(15 - e) with 2^e the
+// power of two at or below that product (without the half) brings |dS| to 2^15 at most: a
+// factor of two from the largest fp16 for what P and delta are off, and all of the range below
+// for small P (undone when acc1 leaves).
 __device__ __forceinline__ float grad_scale(float bound) {
   const unsigned e = __float_as_uint(bound) >> 23;
-  return e < 14 || e >= 0xfe ? 1.f : __uint_as_float((268 - e) << 23);
+  return e < 15 || e >= 0xfe ? 1.f : __uint_as_float((269 - e) << 23);
 }
 
-// The largest |v|^2 of each cloud and kv head, by tiles of keys; rows that are not finite
+// The largest |v|^2 of each tile of keys and kv head, in the slots of its cloud's queries (the last
+// one has all further tiles); rows that are not finite
 // are left out: what they spoil is spoilt whatever the scale is.  A maximum is the same in any
 // order.  Four lanes share a row, and every load of a tile is in flight at once: 9.5 us for two
 // clouds of 4096 to 8192 tokens, 8 heads of width 128 (0.4 % of the backward), 3 us for small ones.
@@ -481,7 +482,8 @@ __global__ void __launch_bounds__(128) packed_value_max_kernel(const PackedArgs 
   if (threadIdx.x % 32 == 0) best[threadIdx.x / 32] = bits;
   __syncthreads();
   if (threadIdx.x == 0)
-    atomicMax(reinterpret_cast<unsigned*>(a.v_max) + (int64_t)kvh * (a.H / a.Hk) * a.Tq + t.b0,
+    atomicMax(reinterpret_cast<unsigned*>(a.v_max) + (int64_t)kvh * (a.H / a.Hk) * a.Tq + t.b0 +
+                  min((t.row0 - t.a0) / kTile, t.nb - 1),
               max(max(best[0], best[1]), max(best[2], best[3])));
 }
 
@@ -652,7 +654,10 @@ __global__ void __launch_bounds__(Bwd<DP>::threads, Bwd<DP>::GROUPS == 2 ? 1 : 2
     if (std::is_same<T, __half>::value) {
       // a row of dQ: its own bound; dK: every row's that the block meets
       if (!DKV) {
-        if (live && n > 0) big = a.ds_bound[(int64_t)head0 * a.Tq + t.row0 + row] * sqrtf(a.v_max[(int64_t)kvh * group * a.Tq + t.a0]);
+        const float* tiles = a.v_max + (int64_t)kvh * group * a.Tq + t.a0;
+        for (int i = threadIdx.x % 32; i <= min((c_end - 1) / kTile, t.na - 1); i += 32) big = fmaxf(big, tiles[i]);
+        big = sqrtf(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big))));
+        big *= live && n > 0 ? a.ds_bound[(int64_t)head0 * a.Tq + t.row0 + row] : 0.f;
         if (!(big < INFINITY)) big = 0.f;  // such a row's gradients are not finite whatever the scale is
       } else {
         for (int h = 0; h < group; ++h)
